@@ -14,7 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libvcommit.so")
 
 VC_OK, VC_EINVAL, VC_ENOMEM, VC_ECUDA, VC_ETIMEDOUT, VC_ERANGE, VC_ENOTSUP = range(7)
-VC_DTYPE_BF16, VC_DTYPE_F32, VC_DTYPE_F64 = 0, 1, 2
+VC_DTYPE_BF16, VC_DTYPE_F32, VC_DTYPE_F64, VC_DTYPE_F16 = 0, 1, 2, 3
 VC_ROPE_NONE, VC_ROPE_LLAMA3, VC_ROPE_LINEAR = 0, 1, 2
 
 SYMBOLS = (
@@ -23,6 +23,7 @@ SYMBOLS = (
     "vc_build_trees", "vc_prove", "vc_tree_set_count", "vc_tree_nodes", "vc_tree_set_free",
     "vc_int_peak", "vc_wait_probe", "vc_kv_commit_noalloc", "vc_kv_open", "vc_io_extend", "vc_io_genesis",
     "vc_kv_transcript", "vc_kv_transcript_commit",
+    "vc_rope_append", "vc_paged_attention", "vc_paged_attention_workspace",
 )
 
 
@@ -113,6 +114,11 @@ def _declare(lib):
                        POINTER(c_int32)],
         "vc_kv_transcript": [P, POINTER(KvtDesc), P, P],
         "vc_kv_transcript_commit": [P, POINTER(KvtDesc), c_int32, P, POINTER(P)],
+        "vc_rope_append": [P, POINTER(KvDesc), c_int32, c_int32, P, P, c_int32, P, c_int64, c_int64, P, c_int64, c_int64,
+                           P, c_int64, c_int64, P, c_int64, c_int64, P, c_int32, c_double, c_int32],
+        "vc_paged_attention": [P, POINTER(KvDesc), c_int32, c_int32, c_int32, c_int32, P, c_int64, c_int64, c_int64,
+                               P, c_double, P, P, P, c_size_t],
+        "vc_paged_attention_workspace": [P, POINTER(KvDesc), c_int32, c_int32, POINTER(c_size_t)],
     }.items():
         fn = getattr(lib, name)
         fn.restype = c_int32

@@ -1063,6 +1063,187 @@ vc_status vc_kv_transcript_commit(vc_ctx* c, const vc_kvt_desc* d, int32_t layer
   return VC_OK;
 }
 
+// -------------------------------------------------------------- decode step
+
+namespace {
+
+// A paged cache that the decode-step calls can address.
+vc_status check_paged(const vc_kv_desc* d, int32_t layer, const char* fn) {
+  if (!d->block_tables) return fail(VC_ENOTSUP, "%s: the cache must be paged (block_tables is NULL)", fn);
+  if (d->dtype != VC_DTYPE_BF16 && d->dtype != VC_DTYPE_F16 && d->dtype != VC_DTYPE_F32)
+    return fail(VC_ENOTSUP, "%s: dtype %d is not bf16, f16 or f32", fn, d->dtype);
+  if (d->n_layers < 1 || d->n_seqs < 1 || d->n_kv_heads < 1 || d->block_size < 1 || d->max_blocks_per_seq < 1)
+    return fail(VC_EINVAL, "%s: n_layers, n_seqs, n_kv_heads, block_size and max_blocks_per_seq must be >= 1", fn);
+  if (layer < 0 || layer >= d->n_layers) return fail(VC_ERANGE, "%s: layer %d of %d", fn, layer, d->n_layers);
+  if (d->head_dim < 2 || d->head_dim > 256 || d->head_dim % 2)
+    return fail(VC_ENOTSUP, "%s: head_dim %d is not even or not in [2, 256]", fn, d->head_dim);
+  if (d->cache_elems <= 0) return fail(VC_EINVAL, "%s: cache_elems must be > 0", fn);
+  const int64_t top = int64_t(1) << 31;     // page * stride_page + slot * stride_row stays in 63 bits
+  if (d->stride_page < 0 || d->stride_row < 0 || d->stride_head < 0 || d->stride_page >= top || d->stride_row >= top ||
+      d->stride_head >= top)
+    return fail(VC_EINVAL, "%s: cache strides must be in [0, 2^31)", fn);
+  if (!d->k_layers || !d->v_layers || !d->k_layers[layer] || !d->v_layers[layer])
+    return fail(VC_EINVAL, "%s: NULL K/V pointer of layer %d", fn, layer);
+  const int esz = d->dtype == VC_DTYPE_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(d->k_layers[layer]) % esz || reinterpret_cast<uintptr_t>(d->v_layers[layer]) % esz)
+    return fail(VC_EINVAL, "%s: K/V base of layer %d not aligned to its element size", fn, layer);
+  return VC_OK;
+}
+
+int64_t paged_row_span(const vc_kv_desc* d) { return int64_t(d->n_kv_heads - 1) * d->stride_head + d->head_dim; }
+
+vc_status check_rows(const void* p, int esz, const char* fn, const char* name) {
+  if (!p) return fail(VC_EINVAL, "%s: %s is NULL", fn, name);
+  if (reinterpret_cast<uintptr_t>(p) % esz) return fail(VC_EINVAL, "%s: %s not aligned to its element size", fn, name);
+  return VC_OK;
+}
+
+vc_status check_attn(const vc_kv_desc* d, int32_t layer, int32_t n_new, int32_t n_heads, const char* fn) {
+  vc_status r = check_paged(d, layer, fn);
+  if (r) return r;
+  if (n_new < 1 || n_heads < 1) return fail(VC_EINVAL, "%s: n_new and n_heads must be >= 1", fn);
+  if (n_heads % d->n_kv_heads)
+    return fail(VC_EINVAL, "%s: %d query heads are no multiple of %d KV heads", fn, n_heads, d->n_kv_heads);
+  if (int64_t(n_new) * (n_heads / d->n_kv_heads) > 65535)
+    return fail(VC_ENOTSUP, "%s: more than 65535 query rows of one KV head", fn);
+  return VC_OK;
+}
+
+void fill_attn(AttnArgs* a, const vc_kv_desc* d, int32_t layer, int32_t n_new, int32_t n_heads) {
+  std::memset(a, 0, sizeof(*a));
+  a->n_new = n_new;
+  a->n_heads = n_heads;
+  a->n_kv_heads = d->n_kv_heads;
+  a->head_dim = d->head_dim;
+  a->rows = n_new * (n_heads / d->n_kv_heads);
+  a->k = d->k_layers[layer];
+  a->v = d->v_layers[layer];
+  a->block_tables = d->block_tables;
+  a->max_blocks = d->max_blocks_per_seq;
+  a->block_size = d->block_size;
+  a->stride_page = d->stride_page;
+  a->stride_row = d->stride_row;
+  a->stride_head = d->stride_head;
+  a->cache_elems = d->cache_elems;
+  a->row_span = paged_row_span(d);
+}
+
+}  // namespace
+
+vc_status vc_rope_append(vc_ctx* c, const vc_kv_desc* d, int32_t layer, int32_t n_tokens, const int32_t* positions,
+                         const int32_t* seq_ids, int32_t n_heads, const void* q, int64_t q_tok, int64_t q_head,
+                         void* q_out, int64_t qo_tok, int64_t qo_head, const void* k, int64_t k_tok, int64_t k_head,
+                         const void* v, int64_t v_tok, int64_t v_head, const double* inv_freq, int32_t rotary_dim,
+                         double factor, int32_t neighbours) {
+  if (!c || !d) return fail(VC_EINVAL, "vc_rope_append: NULL argument");
+  vc_status r = check_paged(d, layer, "vc_rope_append");
+  if (r) return r;
+  if (n_tokens < 0 || n_heads < 1) return fail(VC_EINVAL, "vc_rope_append: n_tokens must be >= 0 and n_heads >= 1");
+  if (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > d->head_dim)
+    return fail(VC_EINVAL, "vc_rope_append: rotary_dim %d is odd or not in [2, head_dim]", rotary_dim);
+  if ((d->n_kv_heads > 1 && d->stride_head < d->head_dim) || (d->block_size > 1 && d->stride_row < d->head_dim))
+    return fail(VC_EINVAL, "vc_rope_append: the cache's rows or heads overlap");
+  if (!seq_ids && n_tokens > d->n_seqs)
+    return fail(VC_EINVAL, "vc_rope_append: %d tokens of %d sequences need seq_ids", n_tokens, d->n_seqs);
+  if (n_tokens == 0) return VC_OK;
+  if (!positions || !inv_freq) return fail(VC_EINVAL, "vc_rope_append: positions or inv_freq is NULL");
+  const int esz = d->dtype == VC_DTYPE_F32 ? 4 : 2;
+  r = check_rows(q, esz, "vc_rope_append", "q");
+  if (!r) r = check_rows(q_out, esz, "vc_rope_append", "q_out");
+  if (!r) r = check_rows(k, esz, "vc_rope_append", "k");
+  if (!r) r = check_rows(v, esz, "vc_rope_append", "v");
+  if (r) return r;
+  DeviceGuard g(c->device);
+  RopeArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.n_tokens = n_tokens;
+  a.n_heads = n_heads;
+  a.n_kv_heads = d->n_kv_heads;
+  a.head_dim = d->head_dim;
+  a.rotary_dim = rotary_dim;
+  a.neighbours = neighbours != 0;
+  a.positions = positions;
+  a.seq_ids = seq_ids;
+  a.inv_freq = inv_freq;
+  a.factor = factor;
+  a.q = q, a.q_tok = q_tok, a.q_head = q_head;
+  a.q_out = q_out, a.qo_tok = qo_tok, a.qo_head = qo_head;
+  a.k = k, a.k_tok = k_tok, a.k_head = k_head;
+  a.v = v, a.v_tok = v_tok, a.v_head = v_head;
+  a.k_cache = const_cast<void*>(d->k_layers[layer]);
+  a.v_cache = const_cast<void*>(d->v_layers[layer]);
+  a.block_tables = d->block_tables;
+  a.n_seqs = d->n_seqs;
+  a.max_blocks = d->max_blocks_per_seq;
+  a.block_size = d->block_size;
+  a.stride_page = d->stride_page;
+  a.stride_row = d->stride_row;
+  a.stride_head = d->stride_head;
+  a.cache_elems = d->cache_elems;
+  a.row_span = paged_row_span(d);
+  a.err = c->err;
+  const cudaError_t e = launch_rope_append(a, d->dtype, rope_chunk_width(a, esz), c->n_sm, c->stream);
+  if (e != cudaSuccess) return fail(VC_ECUDA, "vc_rope_append launch: %s", cudaGetErrorString(e));
+  return VC_OK;
+}
+
+vc_status vc_paged_attention_workspace(vc_ctx* c, const vc_kv_desc* d, int32_t n_new, int32_t n_heads,
+                                       size_t* bytes_out) {
+  if (!c || !d || !bytes_out) return fail(VC_EINVAL, "vc_paged_attention_workspace: NULL argument");
+  vc_status r = check_attn(d, 0, n_new, n_heads, "vc_paged_attention_workspace");
+  if (r) return r;
+  DeviceGuard g(c->device);
+  AttnArgs a;
+  fill_attn(&a, d, 0, n_new, n_heads);
+  size_t bytes = 0;
+  const cudaError_t e = paged_attn_workspace(a, d->dtype, c->n_sm, &bytes);
+  if (e != cudaSuccess) return fail(VC_ECUDA, "vc_paged_attention_workspace: %s", cudaGetErrorString(e));
+  *bytes_out = bytes;
+  return VC_OK;
+}
+
+vc_status vc_paged_attention(vc_ctx* c, const vc_kv_desc* d, int32_t layer, int32_t n_seqs, int32_t n_new,
+                             int32_t n_heads, const void* q, int64_t q_seq, int64_t q_tok, int64_t q_head,
+                             const int32_t* seq_lens, double scale, void* out, float* lse, void* workspace,
+                             size_t workspace_bytes) {
+  if (!c || !d) return fail(VC_EINVAL, "vc_paged_attention: NULL argument");
+  vc_status r = check_attn(d, layer, n_new, n_heads, "vc_paged_attention");
+  if (r) return r;
+  if (n_seqs < 0 || n_seqs > d->n_seqs)
+    return fail(VC_EINVAL, "vc_paged_attention: %d sequences, the block table has %d", n_seqs, d->n_seqs);
+  if (int64_t(n_seqs) * d->n_kv_heads > 0x7FFFFFFF)
+    return fail(VC_ENOTSUP, "vc_paged_attention: too many (sequence, KV head) pairs");
+  if (!(scale > -1e30 && scale < 1e30)) return fail(VC_EINVAL, "vc_paged_attention: scale is not finite");
+  if (n_seqs == 0) return VC_OK;
+  if (!seq_lens) return fail(VC_EINVAL, "vc_paged_attention: seq_lens is NULL");
+  const int esz = d->dtype == VC_DTYPE_F32 ? 4 : 2;
+  r = check_rows(q, esz, "vc_paged_attention", "q");
+  if (!r) r = check_rows(out, esz, "vc_paged_attention", "out");
+  if (!r && lse) r = check_rows(lse, 4, "vc_paged_attention", "lse");
+  if (!r) r = check_rows(workspace, 16, "vc_paged_attention", "workspace");
+  if (r) return r;
+  DeviceGuard g(c->device);
+  AttnArgs a;
+  fill_attn(&a, d, layer, n_new, n_heads);
+  a.n_seqs = n_seqs;
+  a.q = q, a.q_seq = q_seq, a.q_tok = q_tok, a.q_head = q_head;
+  a.seq_lens = seq_lens;
+  a.scale_log2 = float(scale * 1.4426950408889634);
+  a.out = out;
+  a.lse = lse;
+  a.parts = static_cast<float*>(workspace);
+  a.err = c->err;
+  AttnPlan plan;
+  cudaError_t e = plan_paged_attn(a, d->dtype, c->n_sm, &plan);
+  if (e != cudaSuccess) return fail(VC_ECUDA, "vc_paged_attention: %s", cudaGetErrorString(e));
+  if (workspace_bytes < plan.workspace)
+    return fail(VC_EINVAL, "vc_paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, plan.workspace);
+  a.n_workers = plan.n_workers;
+  e = launch_paged_attn(a, plan, c->stream);
+  if (e != cudaSuccess) return fail(VC_ECUDA, "vc_paged_attention launch: %s", cudaGetErrorString(e));
+  return VC_OK;
+}
+
 vc_status vc_int_peak(vc_ctx* c, int32_t variant, int64_t iters, double* ops_per_s) {
   if (!c || !ops_per_s || iters < 1 || variant < 0 || variant > 3) return fail(VC_EINVAL, "vc_int_peak: bad argument");
   DeviceGuard g(c->device);

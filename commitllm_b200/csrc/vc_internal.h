@@ -159,6 +159,52 @@ struct KvtcArgs {
 bool kvt_commit_supported(int head_dim, int kv_dim);
 cudaError_t launch_kvt_commit(const KvtcArgs& a, int n_sm, cudaStream_t s);
 
+// rope_append.cu
+struct RopeArgs {
+  int32_t n_tokens, n_heads, n_kv_heads, head_dim, rotary_dim, neighbours;
+  const int32_t* positions;    // [n_tokens]; < 0: padding
+  const int32_t* seq_ids;      // [n_tokens], or nullptr: token t belongs to sequence t
+  const double* inv_freq;      // [rotary_dim / 2]
+  double factor;               // on cos and sin
+  const void* q; int64_t q_tok, q_head;
+  void* q_out; int64_t qo_tok, qo_head;
+  const void* k; int64_t k_tok, k_head;
+  const void* v; int64_t v_tok, v_head;
+  void* k_cache; void* v_cache;
+  const int32_t* block_tables; int32_t n_seqs, max_blocks, block_size;
+  int64_t stride_page, stride_row, stride_head;   // elements
+  int64_t cache_elems, row_span;
+  int* err;
+};
+int rope_chunk_width(const RopeArgs& a, int esz);
+cudaError_t launch_rope_append(const RopeArgs& a, int dtype, int width, int n_sm, cudaStream_t s);
+
+// paged_attn.cu
+struct AttnArgs {
+  int32_t n_seqs, n_new, n_heads, n_kv_heads, head_dim;
+  int32_t rows;                // query rows of one KV head: n_new * n_heads / n_kv_heads
+  const void* q; int64_t q_seq, q_tok, q_head;
+  const void* k; const void* v;
+  const int32_t* block_tables; int32_t max_blocks, block_size;
+  int64_t stride_page, stride_row, stride_head;   // elements
+  int64_t cache_elems, row_span;
+  const int32_t* seq_lens;     // [n_seqs]
+  float scale_log2;            // scale * log2(e)
+  void* out;                   // [n_seqs][n_new][n_heads][head_dim]
+  float* lse;                  // [n_seqs][n_new][n_heads] or nullptr
+  float* parts;                // partial results of split units
+  int32_t n_workers;
+  int* err;
+};
+struct AttnPlan {
+  int variant;                 // index of the kernel
+  int n_workers;               // CTAs
+  size_t workspace;            // bytes of parts
+};
+cudaError_t paged_attn_workspace(const AttnArgs& a, int dtype, int n_sm, size_t* bytes);
+cudaError_t plan_paged_attn(const AttnArgs& a, int dtype, int n_sm, AttnPlan* plan);
+cudaError_t launch_paged_attn(const AttnArgs& a, const AttnPlan& plan, cudaStream_t s);
+
 // int_peak.cu
 cudaError_t launch_int_peak(int variant, int64_t iters, int n_sm, uint32_t* sink, cudaStream_t s,
                             double* ops_per_launch);

@@ -54,6 +54,7 @@ typedef int32_t vc_status;
 #define VC_DTYPE_BF16 0 /* raw bf16 bits, widened exactly to f64 before hashing */
 #define VC_DTYPE_F32 1  /* f32, widened exactly to f64 */
 #define VC_DTYPE_F64 2  /* f64 as the reference's KvEntry holds it */
+#define VC_DTYPE_F16 3  /* IEEE half; decode-step calls only (the commit calls refuse it) */
 
 typedef struct vc_ctx vc_ctx;           /* per-stream context (scratch, staging) */
 typedef struct vc_tree_set vc_tree_set; /* device-resident Merkle trees */
@@ -381,6 +382,67 @@ VC_API vc_status vc_kv_transcript(vc_ctx* ctx, const vc_kvt_desc* desc, double* 
  */
 VC_API vc_status vc_kv_transcript_commit(vc_ctx* ctx, const vc_kvt_desc* desc, int32_t layer_base,
                                          uint8_t* kv_roots_dev, vc_tree_set** trees_out);
+
+/* -------------------------------------------------------------- decode step */
+
+/*
+ * The serving step over the paged cache that vc_kv_commit hashes (no
+ * counterpart in the reference, whose engine runs these inside vLLM).  `cache`
+ * is a paged vc_kv_desc (block_tables set; VC_ENOTSUP otherwise) of
+ * VC_DTYPE_BF16, F16 or F32 rows with an even head_dim of at most 256; its
+ * n_seqs counts the rows of block_tables; seq_lens, seq_row_offset, layer_base,
+ * pos_base and tree_log2 are not read: lengths and positions are DEVICE arrays,
+ * so that a captured CUDA graph can be replayed as they grow.  stride_page,
+ * stride_row and stride_head must be below 2^31 elements.  Row tensors (q, k,
+ * v, q_out) share the cache's element type, are contiguous within a head, and
+ * have any strides (in elements) between heads and tokens.  These calls
+ * allocate nothing, copy nothing from the host and never synchronise: they can
+ * be captured.  A page id, position or sequence that leaves the table or the
+ * cache is reported by the next vc_ctx_sync as VC_ERANGE; that row is not
+ * touched.
+ */
+
+/*
+ * Rotary positions of n_tokens tokens, K and V rows into their pages.  Token t
+ * of sequence seq_ids_dev[t] (NULL: sequence t) at position p =
+ * positions_dev[t]: pair i < rotary_dim / 2 of every q and k head, elements
+ * (i, i + rotary_dim / 2), or (2i, 2i + 1) if neighbours != 0, is turned by
+ * p * inv_freq_dev[i] (DEVICE f64; angle, cos and sin in f64) and multiplied by
+ * `factor`; elements from rotary_dim on are kept.  q goes to q_out (which may
+ * be q itself), k and v to row p of the sequence.  p < 0 marks padding: q is
+ * copied unchanged and no row is written.  Two tokens of one call must not
+ * share a row: that row would hold a mix of both.
+ */
+VC_API vc_status vc_rope_append(vc_ctx* ctx, const vc_kv_desc* cache, int32_t layer, int32_t n_tokens,
+                                const int32_t* positions_dev, const int32_t* seq_ids_dev, int32_t n_heads,
+                                const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                                void* q_out, int64_t qo_tok_stride, int64_t qo_head_stride,
+                                const void* k, int64_t k_tok_stride, int64_t k_head_stride,
+                                const void* v, int64_t v_tok_stride, int64_t v_head_stride,
+                                const double* inv_freq_dev, int32_t rotary_dim, double factor, int32_t neighbours);
+
+/*
+ * Attention of the n_new newest tokens of each of the first n_seqs sequences.
+ * With n = seq_lens_dev[s] cached rows, the new tokens' own among them, token j
+ * sees rows p < n - n_new + 1 + j:
+ *   out[s][j][h] = sum_p softmax_p(scale * q[s][j][h] . k_p) v_p
+ * over the rows of KV head h / (n_heads / n_kv_heads); lse_dev[s][j][h] (NULL:
+ * not wanted) = log sum_p exp(scale * q . k_p).  A token that sees no row gets
+ * zeros and -infinity; rows a token does not see cannot reach its output,
+ * whatever they hold.  Scores, sums and outputs are accumulated in f32 and
+ * rounded once.  out: DEVICE [n_seqs][n_new][n_heads][head_dim]; lse: f32
+ * [n_seqs][n_new][n_heads].  workspace_dev: DEVICE, 16-byte aligned, of at least
+ * vc_paged_attention_workspace bytes; a call that may run at the same time (a
+ * graph replayed on another stream) needs its own.
+ */
+VC_API vc_status vc_paged_attention(vc_ctx* ctx, const vc_kv_desc* cache, int32_t layer, int32_t n_seqs,
+                                    int32_t n_new, int32_t n_heads, const void* q, int64_t q_seq_stride,
+                                    int64_t q_tok_stride, int64_t q_head_stride, const int32_t* seq_lens_dev,
+                                    double scale, void* out, float* lse_dev, void* workspace_dev,
+                                    size_t workspace_bytes);
+/* Bytes of workspace that vc_paged_attention needs for any call with this cache, n_new and n_heads. */
+VC_API vc_status vc_paged_attention_workspace(vc_ctx* ctx, const vc_kv_desc* cache, int32_t n_new, int32_t n_heads,
+                                              size_t* bytes_out);
 
 /* --------------------------------------------------------- measurement aid */
 

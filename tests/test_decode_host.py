@@ -1,0 +1,54 @@
+"""Host side of the decode-step operators: rope frequencies, and refusals that need no GPU."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+from commitllm_b200 import _lib
+from commitllm_b200 import commit as C
+from commitllm_b200 import decode as D
+from oracle import commit_oracle as O
+
+
+@pytest.mark.parametrize("scaling", [None, "linear", "llama3"])
+@pytest.mark.parametrize("dim", [16, 64, 128])
+def test_frequencies_equal_the_transcripts(scaling, dim):
+    """The scalings that the KV transcript has: every f64 equal to the oracle's."""
+    cfg = C.RopeConfig(theta=500000.0, scaling=scaling)
+    inv, factor = D.rope_frequencies(cfg, dim)
+    want = O.scaled_inv_freq(dim, 500000.0, O.RopeScaling(rope_type=scaling) if scaling else None)
+    assert factor == 1.0
+    assert np.array_equal(np.asarray(inv), np.asarray(want))
+
+
+def test_yarn_frequencies():
+    cfg = C.RopeConfig(theta=10000.0, scaling="yarn", factor=16.0, original_max_position_embeddings=4096)
+    inv, factor = D.rope_frequencies(cfg, 128)
+    plain = [10000.0 ** (-2 * i / 128) for i in range(64)]
+    assert factor == 0.1 * math.log(16.0) + 1.0
+    assert np.allclose(inv[:16], plain[:16], rtol=1e-15) and np.allclose(inv[-10:], np.asarray(plain[-10:]) / 16, rtol=1e-15)
+    assert all(a >= b for a, b in zip(inv, inv[1:]))
+    # between the ends: a pair that turns t times in the original length is part stretched
+    i = 30
+    lo = math.floor(128 * math.log(4096 / (32 * 2 * math.pi)) / (2 * math.log(10000.0)))
+    hi = math.ceil(128 * math.log(4096 / (2 * math.pi)) / (2 * math.log(10000.0)))
+    s = (i - lo) / (hi - lo)
+    assert 0 < s < 1 and inv[i] == pytest.approx(plain[i] * (1 - s) + plain[i] / 16 * s, rel=1e-15)
+    assert D.rope_frequencies(cfg, 128, attention_factor=1.0)[1] == 1.0
+
+
+@pytest.mark.parametrize("cfg,dim", [(C.RopeConfig(scaling="other"), 64), (C.RopeConfig(), 7), (C.RopeConfig(), 0),
+                                     (C.RopeConfig(theta=0.0), 64), (C.RopeConfig(scaling="linear", factor=0.0), 64)])
+def test_frequency_refusals(cfg, dim):
+    with pytest.raises(ValueError):
+        D.rope_frequencies(cfg, dim)
+
+
+def test_entry_points_refuse_null_arguments():
+    lib = _lib.lib()
+    assert lib.vc_rope_append(None, None, 0, 0, None, None, 0, None, 0, 0, None, 0, 0, None, 0, 0, None, 0, 0, None, 0,
+                              1.0, 0) == _lib.VC_EINVAL
+    assert lib.vc_paged_attention(None, None, 0, 0, 0, 0, None, 0, 0, 0, None, 1.0, None, None, None, 0) == _lib.VC_EINVAL
+    out = ctypes.c_size_t()
+    assert lib.vc_paged_attention_workspace(None, None, 0, 0, ctypes.byref(out)) == _lib.VC_EINVAL
