@@ -24,6 +24,7 @@ SYMBOLS = (
     "vc_int_peak", "vc_wait_probe", "vc_kv_commit_noalloc", "vc_kv_open", "vc_io_extend", "vc_io_genesis",
     "vc_kv_transcript", "vc_kv_transcript_commit",
     "vc_rope_append", "vc_paged_attention", "vc_paged_attention_workspace",
+    "vc_verify_tokens", "vc_verify_tokens_workspace",
 )
 
 
@@ -119,6 +120,9 @@ def _declare(lib):
         "vc_paged_attention": [P, POINTER(KvDesc), c_int32, c_int32, c_int32, c_int32, P, c_int64, c_int64, c_int64,
                                P, c_double, P, P, P, c_size_t],
         "vc_paged_attention_workspace": [P, POINTER(KvDesc), c_int32, c_int32, POINTER(c_size_t)],
+        "vc_verify_tokens": [P, c_int32, c_int32, c_int32, P, c_int32, c_int64, c_int64, P, c_int64, c_int64, P, P, P,
+                             P, P, P, c_size_t],
+        "vc_verify_tokens_workspace": [P, c_int32, c_int32, c_int32, POINTER(c_size_t)],
     }.items():
         fn = getattr(lib, name)
         fn.restype = c_int32

@@ -17,7 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libvcommit.so")
-SOURCES = ["merkle.cu", "trace.cu", "kv_transcript.cu", "kvt_commit.cu", "rope_append.cu", "paged_attn.cu",
+SOURCES = ["merkle.cu", "trace.cu", "kv_transcript.cu", "kvt_commit.cu", "rope_append.cu", "paged_attn.cu", "verify.cu",
            "int_peak.cu", "api.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",

@@ -1244,6 +1244,66 @@ vc_status vc_paged_attention(vc_ctx* c, const vc_kv_desc* d, int32_t layer, int3
   return VC_OK;
 }
 
+static vc_status plan_verify_call(vc_ctx* c, int32_t n_seqs, int32_t n_draft, int32_t vocab, VerifyArgs* a,
+                                  size_t* bytes, const char* fn) {
+  if (n_seqs < 0 || n_draft < 0 || vocab < 1) return fail(VC_EINVAL, "%s: n_seqs, n_draft must be >= 0 and vocab >= 1", fn);
+  if (vocab > (1 << 20)) return fail(VC_ENOTSUP, "%s: vocab %d above 2^20", fn, vocab);
+  if (int64_t(n_seqs) * (int64_t(n_draft) + 1) > (int64_t(1) << 26) || int64_t(n_seqs) > (int64_t(1) << 26))
+    return fail(VC_ENOTSUP, "%s: more than 2^26 logits rows", fn);
+  std::memset(a, 0, sizeof(*a));
+  a->n_seqs = n_seqs;
+  a->n_draft = n_draft;
+  a->vocab = vocab;
+  *bytes = 0;
+  if (n_seqs == 0) return VC_OK;
+  plan_verify(a, c->n_sm);
+  *bytes = size_t(n_seqs) * size_t(n_draft + 1) * size_t(a->splits) * sizeof(VerifyPart);
+  return VC_OK;
+}
+
+vc_status vc_verify_tokens_workspace(vc_ctx* c, int32_t n_seqs, int32_t n_draft, int32_t vocab, size_t* bytes_out) {
+  if (!c || !bytes_out) return fail(VC_EINVAL, "vc_verify_tokens_workspace: NULL argument");
+  VerifyArgs a;
+  return plan_verify_call(c, n_seqs, n_draft, vocab, &a, bytes_out, "vc_verify_tokens_workspace");
+}
+
+vc_status vc_verify_tokens(vc_ctx* c, int32_t n_seqs, int32_t n_draft, int32_t vocab, const void* logits,
+                           int32_t logits_dtype, int64_t logits_seq, int64_t logits_tok, const float* draft_probs,
+                           int64_t probs_seq, int64_t probs_tok, const int32_t* drafts, const double* uniforms,
+                           const float* temperature, int32_t* tokens, int32_t* counts, void* workspace,
+                           size_t workspace_bytes) {
+  if (!c) return fail(VC_EINVAL, "vc_verify_tokens: NULL argument");
+  VerifyArgs a;
+  size_t need = 0;
+  vc_status r = plan_verify_call(c, n_seqs, n_draft, vocab, &a, &need, "vc_verify_tokens");
+  if (r || n_seqs == 0) return r;
+  if (logits_dtype != VC_DTYPE_BF16 && logits_dtype != VC_DTYPE_F16 && logits_dtype != VC_DTYPE_F32)
+    return fail(VC_ENOTSUP, "vc_verify_tokens: logits dtype %d is not bf16, f16 or f32", logits_dtype);
+  r = check_rows(logits, logits_dtype == VC_DTYPE_F32 ? 4 : 2, "vc_verify_tokens", "logits");
+  if (!r && n_draft) r = check_rows(drafts, 4, "vc_verify_tokens", "drafts");
+  if (!r && draft_probs) r = check_rows(draft_probs, 4, "vc_verify_tokens", "draft_probs");
+  if (!r) r = check_rows(uniforms, 8, "vc_verify_tokens", "uniforms");
+  if (!r) r = check_rows(temperature, 4, "vc_verify_tokens", "temperature");
+  if (!r) r = check_rows(tokens, 4, "vc_verify_tokens", "tokens");
+  if (!r) r = check_rows(counts, 4, "vc_verify_tokens", "counts");
+  if (!r) r = check_rows(workspace, 16, "vc_verify_tokens", "workspace");
+  if (r) return r;
+  if (workspace_bytes < need)
+    return fail(VC_EINVAL, "vc_verify_tokens: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  DeviceGuard g(c->device);
+  a.logits = logits, a.logits_seq = logits_seq, a.logits_tok = logits_tok;
+  a.draft_probs = n_draft ? draft_probs : nullptr, a.probs_seq = probs_seq, a.probs_tok = probs_tok;
+  a.drafts = drafts;
+  a.uniforms = uniforms;
+  a.temperature = temperature;
+  a.parts = static_cast<VerifyPart*>(workspace);
+  a.tokens = tokens;
+  a.counts = counts;
+  const cudaError_t e = launch_verify(a, logits_dtype, c->stream);
+  if (e != cudaSuccess) return fail(VC_ECUDA, "vc_verify_tokens launch: %s", cudaGetErrorString(e));
+  return VC_OK;
+}
+
 vc_status vc_int_peak(vc_ctx* c, int32_t variant, int64_t iters, double* ops_per_s) {
   if (!c || !ops_per_s || iters < 1 || variant < 0 || variant > 3) return fail(VC_EINVAL, "vc_int_peak: bad argument");
   DeviceGuard g(c->device);

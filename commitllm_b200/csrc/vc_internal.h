@@ -205,6 +205,29 @@ cudaError_t paged_attn_workspace(const AttnArgs& a, int dtype, int n_sm, size_t*
 cudaError_t plan_paged_attn(const AttnArgs& a, int dtype, int n_sm, AttnPlan* plan);
 cudaError_t launch_paged_attn(const AttnArgs& a, const AttnPlan& plan, cudaStream_t s);
 
+// verify.cu
+struct VerifyPart {            // one slice of a logits row
+  double s, b;                 // sum of the weights relative to m, and of those before the draft
+  float m;                     // maximum
+  int32_t best;                // its lowest index
+  int32_t bad;                 // a NaN was seen
+  int32_t pad_;
+};
+struct VerifyArgs {
+  int32_t n_seqs, n_draft, vocab;
+  const void* logits; int64_t logits_seq, logits_tok;          // elements
+  const float* draft_probs; int64_t probs_seq, probs_tok;      // or nullptr
+  const int32_t* drafts;       // [n_seqs][n_draft]
+  const double* uniforms;      // [n_seqs][n_draft + 1]
+  const float* temperature;    // [n_seqs]
+  VerifyPart* parts;           // [n_seqs * (n_draft + 1)][splits]
+  int32_t slice, splits;
+  int32_t* tokens;             // [n_seqs][n_draft + 1]
+  int32_t* counts;             // [n_seqs]
+};
+void plan_verify(VerifyArgs* a, int n_sm);
+cudaError_t launch_verify(const VerifyArgs& a, int dtype, cudaStream_t s);
+
 // int_peak.cu
 cudaError_t launch_int_peak(int variant, int64_t iters, int n_sm, uint32_t* sink, cudaStream_t s,
                             double* ops_per_launch);

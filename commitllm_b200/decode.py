@@ -304,3 +304,70 @@ def paged_attention(cache: PagedCache, layer: int, q: torch.Tensor, seq_lens: to
                                        None if lse is None else lse.data_ptr(), workspace.data_ptr(),
                                        workspace.numel()))
     return (out, lse) if return_lse else out
+
+
+# ---------------------------------------------------------------------------
+# Drafted tokens
+# ---------------------------------------------------------------------------
+
+def verify_tokens(ctx: Context, logits: torch.Tensor, drafts: torch.Tensor, uniforms: torch.Tensor,
+                  temperature: torch.Tensor, draft_probs: Optional[torch.Tensor] = None,
+                  workspace: Optional[torch.Tensor] = None):
+    """The drafted tokens that the target keeps and the token after them.
+
+    logits: ``[n_seqs, n_draft + 1, vocab]`` float32, bfloat16 or float16, row i
+    the target's at draft i (any strides between rows); drafts: int32 ``[n_seqs,
+    n_draft]`` (a value outside the vocabulary, such as -1, ends a sequence's
+    drafts); uniforms: float64 ``[n_seqs, n_draft + 1]`` in [0, 1); temperature:
+    float32 ``[n_seqs]``, 0 for greedy.  With ``draft_probs`` (float32 ``[n_seqs,
+    n_draft, vocab]``, the distributions the drafts were drawn from) draft i is kept
+    while ``uniforms[i] * q_i(x_i) < p_i(x_i)``, and the next token is drawn with
+    the last uniform from ``max(p - q, 0)`` where a draft was refused, else from
+    ``p``.  Without, the token at i is the one ``p_i`` gives for ``uniforms[i]``, and
+    drafts are kept while they equal it: the tokens are then those of one-by-one
+    decoding, whatever was drafted.  A draw from weights w is the lowest v whose
+    running sum passes ``u * sum(w)``.
+
+    Returns ``(tokens int32 [n_seqs, n_draft + 1], counts int32 [n_seqs])``: each
+    sequence's new tokens, padded with -1.  A reached row with a NaN, a +inf or
+    nothing above -inf ends its sequence without a drawn token.  Rejected drafts'
+    K/V rows stay in their pages until the next step writes them; commit with the
+    lengths that ``counts`` gives.
+    """
+    _on(ctx, logits, "logits")
+    if logits.dtype not in _CACHE_DTYPES or logits.dim() != 3 or 0 in logits.shape[1:]:
+        raise ValueError("logits must be float32, bfloat16 or float16 [n_seqs, n_draft + 1, vocab]")
+    S, N, V = logits.shape
+    ls = logits.stride()
+    if ls[2] != 1 and V > 1:
+        raise ValueError("logits must be contiguous within a row")
+    x = _index(ctx, drafts, "drafts", (S, N - 1))
+    _on(ctx, uniforms, "uniforms")
+    if uniforms.dtype != torch.float64 or uniforms.shape != (S, N) or not uniforms.is_contiguous():
+        raise ValueError(f"uniforms must be contiguous float64 [{S}, {N}]")
+    _on(ctx, temperature, "temperature")
+    if temperature.dtype != torch.float32 or temperature.shape != (S,) or not temperature.is_contiguous():
+        raise ValueError(f"temperature must be contiguous float32 [{S}]")
+    probs, ps = None, (0, 0)
+    if draft_probs is not None:
+        _on(ctx, draft_probs, "draft_probs")
+        ps = draft_probs.stride()
+        if draft_probs.dtype != torch.float32 or draft_probs.shape != (S, N - 1, V) or (ps[2] != 1 and V > 1):
+            raise ValueError(f"draft_probs must be float32 [{S}, {N - 1}, {V}], contiguous within a row")
+        probs = draft_probs.data_ptr()
+    tokens = _empty(ctx, (S, N), torch.int32)
+    counts = _empty(ctx, (S,), torch.int32)
+    if S == 0:
+        return tokens, counts
+    if workspace is None:
+        need = ctypes.c_size_t()
+        check(lib().vc_verify_tokens_workspace(ctx.handle, S, N - 1, V, ctypes.byref(need)))
+        workspace = _empty(ctx, need.value, torch.uint8)
+    else:
+        _on(ctx, workspace, "workspace")
+        if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+            raise ValueError("workspace must be a contiguous uint8 tensor")
+    check(lib().vc_verify_tokens(ctx.handle, S, N - 1, V, logits.data_ptr(), _CACHE_DTYPES[logits.dtype], ls[0], ls[1],
+                                 probs or None, ps[0], ps[1], x, uniforms.data_ptr(), temperature.data_ptr(),
+                                 tokens.data_ptr(), counts.data_ptr(), workspace.data_ptr(), workspace.numel()))
+    return tokens, counts

@@ -444,6 +444,45 @@ VC_API vc_status vc_paged_attention(vc_ctx* ctx, const vc_kv_desc* cache, int32_
 VC_API vc_status vc_paged_attention_workspace(vc_ctx* ctx, const vc_kv_desc* cache, int32_t n_new, int32_t n_heads,
                                               size_t* bytes_out);
 
+/*
+ * How many drafted tokens the target's logits keep, and the token after them.
+ * logits: DEVICE rows [n_seqs][n_draft + 1][vocab] of logits_dtype
+ * (VC_DTYPE_BF16, F16 or F32; strides in elements, contiguous within a row, vocab
+ * <= 2^20): row i is the target's at draft i, row n_draft the one after the last
+ * draft.  p_i = softmax(row i / temperature[s]); a temperature not above 0 puts
+ * all of p_i on the lowest index of the largest logit.  -infinity rules a token
+ * out.  A draw with u from weights w is the lowest v with w_0 + .. + w_v > u *
+ * sum(w).
+ *
+ * draft_probs non-NULL (DEVICE f32 [n_seqs][n_draft][vocab], the distributions
+ * q_i the drafts were drawn from): draft x_i is kept while uniforms[s][i] *
+ * q_i(x_i) < p_i(x_i); at the first one refused the token is drawn from max(p_i -
+ * q_i, 0), after the last one kept from p_i, both with uniforms[s][n_draft].
+ * draft_probs NULL: the token at position i is drawn from p_i with
+ * uniforms[s][i], and x_i is kept while it equals that token; what comes out is
+ * then what one-by-one decoding with the same numbers gives, drafts or not.
+ * A draft outside [0, vocab) ends the sequence's drafts: the token at its
+ * position is drawn from p_i.
+ *
+ * tokens_dev: DEVICE [n_seqs][n_draft + 1], the kept drafts, the drawn token, then
+ * -1; counts_dev: DEVICE [n_seqs], the tokens of each sequence (drafts kept + 1).
+ * A row that is reached and holds a NaN, a +infinity or nothing above -infinity
+ * ends the sequence without a drawn token (-1, and it is not counted).  Draws
+ * and open comparisons are taken in f64, so the tokens do not depend on how sums
+ * are rounded.  drafts_dev, uniforms_dev (f64 in [0, 1)) and temperature_dev are
+ * contiguous.  workspace_dev: as for vc_paged_attention, of
+ * vc_verify_tokens_workspace bytes.
+ */
+VC_API vc_status vc_verify_tokens(vc_ctx* ctx, int32_t n_seqs, int32_t n_draft, int32_t vocab, const void* logits,
+                                  int32_t logits_dtype, int64_t logits_seq_stride, int64_t logits_tok_stride,
+                                  const float* draft_probs, int64_t probs_seq_stride, int64_t probs_tok_stride,
+                                  const int32_t* drafts_dev, const double* uniforms_dev,
+                                  const float* temperature_dev, int32_t* tokens_dev, int32_t* counts_dev,
+                                  void* workspace_dev, size_t workspace_bytes);
+/* Bytes of workspace that vc_verify_tokens needs. */
+VC_API vc_status vc_verify_tokens_workspace(vc_ctx* ctx, int32_t n_seqs, int32_t n_draft, int32_t vocab,
+                                            size_t* bytes_out);
+
 /* --------------------------------------------------------- measurement aid */
 
 /*

@@ -52,3 +52,6 @@ def test_entry_points_refuse_null_arguments():
     assert lib.vc_paged_attention(None, None, 0, 0, 0, 0, None, 0, 0, 0, None, 1.0, None, None, None, 0) == _lib.VC_EINVAL
     out = ctypes.c_size_t()
     assert lib.vc_paged_attention_workspace(None, None, 0, 0, ctypes.byref(out)) == _lib.VC_EINVAL
+    assert lib.vc_verify_tokens(None, 0, 0, 0, None, 0, 0, 0, None, 0, 0, None, None, None, None, None, None,
+                                0) == _lib.VC_EINVAL
+    assert lib.vc_verify_tokens_workspace(None, 0, 0, 0, ctypes.byref(out)) == _lib.VC_EINVAL
