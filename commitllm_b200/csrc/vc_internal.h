@@ -210,8 +210,6 @@ struct VerifyPart {            // one slice of a logits row
   double s, b;                 // sum of the weights relative to m, and of those before the draft
   float m;                     // maximum
   int32_t best;                // its lowest index
-  int32_t bad;                 // a NaN was seen
-  int32_t pad_;
 };
 struct VerifyArgs {
   int32_t n_seqs, n_draft, vocab;
@@ -222,6 +220,7 @@ struct VerifyArgs {
   const float* temperature;    // [n_seqs]
   VerifyPart* parts;           // [n_seqs * (n_draft + 1)][splits]
   int32_t slice, splits;
+  int32_t wide_logits, wide_probs;   // every row on a 16-byte boundary
   int32_t* tokens;             // [n_seqs][n_draft + 1]
   int32_t* counts;             // [n_seqs]
 };

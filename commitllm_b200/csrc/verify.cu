@@ -36,9 +36,10 @@ constexpr int kMaxCluster = 8;
 
 // How far a keep-or-refuse quantity of the f32 sums may be from its exact value,
 // relative to the row's sum: an exponent of at most 126 (smaller weights are
-// nothing) is rounded three times by 2^-24 of itself, exp2 is off by 2^-22, and
-// a thread's sum of at most 2^7 rounded terms by 2^-17; 126 * 3 * 2^-24 * ln 2 +
-// 2^-22 + 2^-17 < 2.4e-5.
+// nothing) is rounded three times by 2^-24 of itself, exp2 is off by 2^-22, a
+// thread's sum of at most 2^7 rounded terms by 2^-17, and its at most 12 changes
+// of the maximum by 2^-21 each; 126 * 3 * 2^-24 * ln 2 + 2^-22 + 2^-17 + 12 * 2^-21
+// < 3e-5.
 constexpr double kOpen = 4e-5;
 
 template <typename T> __device__ __forceinline__ float to_f32(T x);
@@ -48,43 +49,54 @@ template <> __device__ __forceinline__ float to_f32<__half>(__half x) { return _
 
 __device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
 
-// log2(e) / T, kept finite; 0 for a greedy sequence (T not above 0).
-__device__ __forceinline__ float exponent_scale(float t) { return t > 0.f ? fminf(1.4426950408889634f / t, 3e38f) : 0.f; }
+// log2(e) / T, kept finite and above 0; 1 for a greedy sequence (T not above 0), whose sums nobody reads.
+__device__ __forceinline__ float exponent_scale(float t) {
+  return t > 0.f ? fmaxf(fminf(1.4426950408889634f / t, 3e38f), 1e-37f) : 1.f;
+}
 
+__device__ __forceinline__ float ex2(float x) {      // 2^x within 2^-22 of itself, nothing below 2^-126
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A thread's maximum, sum of exp2((l - m) * c), and the part of it before x.  A NaN
+// or a +infinity leaves a NaN in s (inf - inf), which is how such a row is told.
+template <bool kBefore>
 struct Running {
-  float m = ninf(), s = 0.f, b = 0.f;   // maximum, sum of exp2((l - m) * c), the part of it before x
+  float m = ninf(), s = 0.f, b = 0.f;
   int best = 0x7fffffff;
-  bool bad = false;                     // a NaN
 
-  template <int N>
-  __device__ __forceinline__ void add(const float (&l)[N], int at, float c, int x) {
+  // N elements, of which l[e] is number at + (e / W) * step + e % W
+  template <int N, int W>
+  __device__ __forceinline__ void add(const float (&l)[N], int at, int step, float c, int x) {
     float top = l[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) top = fmaxf(top, l[i]);
     if (top > m) {
-      const float f = m == ninf() ? 0.f : exp2f((m - top) * c);
+      const float f = m == ninf() ? 0.f : ex2((m - top) * c);
       s *= f;
-      b *= f;
+      if (kBefore) b *= f;
       m = top;
-      // the lowest index of the new maximum in this chunk
+      // the lowest index of the new maximum in this batch
 #pragma unroll
       for (int i = N - 1; i >= 0; --i)
-        if (l[i] == top) best = at + i;
+        if (l[i] == top) best = at + (i / W) * step + i % W;
     }
     const float ref = m == ninf() ? 0.f : m;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      bad = bad || l[i] != l[i];
-      const float w = exp2f((l[i] - ref) * c);
+      const float w = ex2((l[i] - ref) * c);
       s += w;
-      if (at + i < x) b += w;
+      if (kBefore && at + (i / W) * step + i % W < x) b += w;
     }
   }
 };
 
-template <typename T>
+template <typename T, bool kBefore>
 __global__ void __launch_bounds__(kStatThreads) verify_stat_kernel(const __grid_constant__ VerifyArgs a) {
   constexpr int N = 16 / sizeof(T);
+  constexpr int kBatch = 4;           // 16-byte loads a thread has under way
   struct alignas(16) Chunk {
     T v[N];
   };
@@ -95,28 +107,38 @@ __global__ void __launch_bounds__(kStatThreads) verify_stat_kernel(const __grid_
   const int hi = min(lo + a.slice, a.vocab);
   const float c = exponent_scale(a.temperature[seq]);
   // without draft probabilities the part of the sum before the draft is wanted
-  const int x = a.draft_probs == nullptr && i < a.n_draft ? a.drafts[int64_t(seq) * a.n_draft + i] : -1;
-  Running r;
+  const int x = kBefore && i < a.n_draft ? a.drafts[int64_t(seq) * a.n_draft + i] : -1;
+  Running<kBefore> r;
   // single elements up to the first 16-byte boundary, chunks, single elements
   const int head = lo < hi ? min(int((16 - (reinterpret_cast<uintptr_t>(src + lo) & 15)) & 15) / int(sizeof(T)), hi - lo) : 0;
   const int body = lo < hi ? (hi - lo - head) / N : 0;
   const int tail = lo + head + body * N;
   if (int(threadIdx.x) < head) {
     const float l[1] = {to_f32(src[lo + threadIdx.x])};
-    r.add(l, lo + threadIdx.x, c, x);
+    r.template add<1, 1>(l, lo + threadIdx.x, 0, c, x);
   }
-#pragma unroll 4
-  for (int j = threadIdx.x; j < body; j += kStatThreads) {
+  int j = threadIdx.x;
+  for (; j + (kBatch - 1) * kStatThreads < body; j += kBatch * kStatThreads) {
+    const int at = lo + head + j * N;
+    Chunk ch[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) ch[k] = *reinterpret_cast<const Chunk*>(src + at + k * kStatThreads * N);
+    float l[kBatch * N];
+#pragma unroll
+    for (int e = 0; e < kBatch * N; ++e) l[e] = to_f32(ch[e / N].v[e % N]);
+    r.template add<kBatch * N, N>(l, at, kStatThreads * N, c, x);
+  }
+  for (; j < body; j += kStatThreads) {
     const int at = lo + head + j * N;
     const Chunk ch = *reinterpret_cast<const Chunk*>(src + at);
     float l[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) l[e] = to_f32(ch.v[e]);
-    r.add(l, at, c, x);
+    r.template add<N, N>(l, at, 0, c, x);
   }
   if (tail + int(threadIdx.x) < hi) {
     const float l[1] = {to_f32(src[tail + threadIdx.x])};
-    r.add(l, tail + threadIdx.x, c, x);
+    r.template add<1, 1>(l, tail + threadIdx.x, 0, c, x);
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // the block's
@@ -127,64 +149,244 @@ __global__ void __launch_bounds__(kStatThreads) verify_stat_kernel(const __grid_
   float m = r.m;
 #pragma unroll
   for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-  const float f = r.m == ninf() ? 0.f : exp2f((r.m - m) * c);
+  // a sum without a maximum is 0 or NaN, and a NaN stays one
+  const float f = r.m == ninf() ? 1.f : ex2((r.m - m) * c);
   double s = double(r.s * f), b = double(r.b * f);
   int best = r.m == m ? r.best : 0x7fffffff;
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
     s += __shfl_xor_sync(~0u, s, d);
-    b += __shfl_xor_sync(~0u, b, d);
+    if (kBefore) b += __shfl_xor_sync(~0u, b, d);
     best = min(best, __shfl_xor_sync(~0u, best, d));
   }
   if (lane == 0) sm[warp] = m, ss[warp] = s, sb[warp] = b, si[warp] = best;
-  const int bad = __syncthreads_or(r.bad);
+  __syncthreads();
   if (threadIdx.x == 0) {
     VerifyPart p{};
     p.m = ninf();
     for (int w = 0; w < kStatThreads / 32; ++w) p.m = fmaxf(p.m, sm[w]);
     p.best = 0x7fffffff;
     for (int w = 0; w < kStatThreads / 32; ++w) {
-      const double g = sm[w] == ninf() ? 0.0 : double(exp2f((sm[w] - p.m) * c));
+      const double g = sm[w] == ninf() ? 1.0 : double(ex2((sm[w] - p.m) * c));
       p.s += g * ss[w];
       p.b += g * sb[w];
       if (sm[w] == p.m) p.best = min(p.best, si[w]);
     }
-    p.bad = bad;
     a.parts[int64_t(row) * a.splits + split] = p;
   }
 }
 
-// One position's joined sums.
+// 2^t in f64 for t <= 0: 2^(j / 64) from a table (shared memory, made by exp2), the
+// rest |r| <= 1 / 128 by the series of 2^r up to r^5 (what follows is below 2^-54).
+// 11 f64 operations, about half of exp(): f64 arithmetic bounds the drawn row.
+constexpr int kTable = 64;
+__device__ __forceinline__ double pow2(double t, const double* table) {
+  if (t < -1000.0) return exp2(t);          // where results lose bits or vanish
+  constexpr double kMagic = 6755399441055744.0;      // 1.5 * 2^52: rounds to a whole number
+  const double z = fma(t, double(kTable), kMagic);
+  const int n = __double2loint(z);
+  const double r = fma(z - kMagic, -1.0 / kTable, t);
+  constexpr double l = 0.693147180559945309417;      // ln 2
+  double p = fma(r, l * l * l * l * l / 120, l * l * l * l / 24);
+  p = fma(r, p, l * l * l / 6);
+  p = fma(r, p, l * l / 2);
+  p = fma(r, p, l);
+  const double v = table[n & (kTable - 1)];
+  p = fma(r * p, v, v);
+  return __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p));
+}
+
+// One position: its row's joined sums, and the draft's weight and probability.
 struct Row {
-  float m;
-  double s, b;     // relative to m
-  int best;
-  bool usable;
+  double s, b;       // relative to m
+  double wx;         // exact
+  float m, qx;
+  int best, x;
+  bool usable, there;
 };
 
-struct Pick {
-  const VerifyArgs& a;
-  cg::cluster_group cl;
-  int seq;
-  double* box;          // this CTA's value for the others
-  double* warp_box;     // [kPickWarps]
-  int* int_box;
-  Row* row_box;
+// The weight of element v of a row: 2^((l - m) log2(e) / T), or what that over the
+// row's sum has above the draft's probability.
+template <typename T>
+struct Weights {
+  const T* l;
+  const float* q;      // nullptr: plain weights
+  const double* table;
+  double m, c, total;
+  bool wide;           // rows on 16-byte boundaries
+  __device__ __forceinline__ double plain(float x) const { return pow2((double(x) - m) * c, table); }
+  __device__ __forceinline__ double of(float x, float qv) const {
+    const double w = plain(x);
+    if (!q) return w;
+    const double d = w / total - double(qv);
+    return d > 0.0 ? d : 0.0;
+  }
+  __device__ __forceinline__ double at(int v) const { return of(to_f32(l[v]), q ? q[v] : 0.f); }
+};
 
-  // Joined by warp 0 of every CTA alike.
-  __device__ Row row(int i) {
-    const int lane = threadIdx.x & 31;
-    if (threadIdx.x < 32) {
-      const float c = exponent_scale(a.temperature[seq]);
+// This CTA's slice [lo, hi) of the vocabulary; its warps hold equal contiguous
+// parts, a multiple of 8 elements but for the last.
+struct Slice {
+  int lo, hi, per_warp;
+};
+
+struct Box {
+  double sum[2];                 // this CTA's sums, for the others: two calls' in turn
+  double warp[kPickWarps];       // its warps'
+  double warp2[kPickWarps];
+  int token;
+};
+
+// Sum of the weights over the slice: all threads get the CTA's, box.warp keeps the parts.
+template <typename T>
+__device__ double slice_sum(const Weights<T>& w, const Slice& sl, Box& box) {
+  constexpr int N = 16 / sizeof(T);
+  struct alignas(16) Chunk {
+    T v[N];
+  };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = min(sl.lo + warp * sl.per_warp, sl.hi), e = min(b + sl.per_warp, sl.hi);
+  double v = 0;
+  int j = b;
+  if (w.wide) {
+    const int n = (e - b) / N;
+#pragma unroll 4
+    for (int k = lane; k < n; k += 32) {
+      const Chunk ch = *reinterpret_cast<const Chunk*>(w.l + b + k * N);
+      float qv[N] = {};
+      if (w.q) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+          *reinterpret_cast<float4*>(qv + i) = *reinterpret_cast<const float4*>(w.q + b + k * N + i);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) v += w.of(to_f32(ch.v[i]), qv[i]);
+    }
+    j = b + n * N;
+  }
+#pragma unroll 4
+  for (j += lane; j < e; j += 32) v += w.at(j);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+  __syncthreads();               // the last call's parts have been read
+  if (lane == 0) box.warp[warp] = v;
+  __syncthreads();
+  double t = 0;
+#pragma unroll
+  for (int x = 0; x < kPickWarps; ++x) t += box.warp[x];
+  return t;
+}
+
+// The first of n consecutive parts whose running sum passes goal, and the sum
+// before it.  Parts' sums are rounded apart from the total that goal comes from, so
+// a goal next to the total may be passed by none: then the last part that still
+// adds to the running sum, not a negligible one behind it.
+__device__ __forceinline__ int first_past(const double* part, int n, double goal, double& before) {
+  double run = before;
+  int at = 0;
+  for (int x = 0; x < n; ++x) {
+    const double next = run + part[x];
+    if (next > run) at = x, before = run;
+    run = next;
+    if (run > goal) break;
+  }
+  return at;
+}
+
+// The lowest v whose running sum passes goal; all[]: the CTAs' sums.  The CTA that
+// holds it calls done(v) from one thread.
+template <typename T, typename Done>
+__device__ void find(const Weights<T>& w, const Slice& sl, Box& box, const double (&all)[kMaxCluster], int n_cta, int me,
+                     double goal, Done done) {
+  double before = 0;
+  if (first_past(all, n_cta, goal, before) != me) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int wp = first_past(box.warp, kPickWarps, goal, before);
+  // that warp's part, cut again over all warps
+  const int b = min(sl.lo + wp * sl.per_warp, sl.hi), e = min(b + sl.per_warp, sl.hi);
+  const int per = (e - b + kPickWarps - 1) / kPickWarps;
+  const int b2 = min(b + warp * per, e), e2 = min(b2 + per, e);
+  double v = 0;
+#pragma unroll 2
+  for (int j = b2 + lane; j < e2; j += 32) v += w.at(j);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+  if (lane == 0) box.warp2[warp] = v;
+  __syncthreads();
+  if (first_past(box.warp2, kPickWarps, goal, before) != warp) return;
+  int token = -1, last = b2;
+  for (int j = b2; j < e2 && token < 0; j += 32) {
+    v = j + lane < e2 ? w.at(j + lane) : 0.0;
+    double incl = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const double o = __shfl_up_sync(~0u, incl, d);
+      if (lane >= d) incl += o;
+    }
+    const double run = before + incl;
+    double prev = __shfl_up_sync(~0u, run, 1);
+    if (lane == 0) prev = before;
+    const unsigned hit = __ballot_sync(~0u, v > 0 && run > goal), adds = __ballot_sync(~0u, run > prev);
+    if (hit) token = j + __ffs(hit) - 1;
+    if (adds) last = j + 31 - __clz(adds);
+    before = __shfl_sync(~0u, run, 31);
+  }
+  if (lane == 0) done(token < 0 ? last : token);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const __grid_constant__ VerifyArgs a) {
+  __shared__ Box box;
+  __shared__ Row rows[kPickWarps];
+  __shared__ double table[kTable];
+  cg::cluster_group cl = cg::this_cluster();
+  const int n_cta = int(cl.num_blocks()), me = int(cl.block_rank());
+  const int seq = blockIdx.x / n_cta;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x < kTable) table[threadIdx.x] = exp2(double(threadIdx.x) / kTable);
+  Slice sl;
+  const int per_cta = ((a.vocab + n_cta - 1) / n_cta + 7) / 8 * 8;
+  sl.lo = min(me * per_cta, a.vocab);
+  sl.hi = min(sl.lo + per_cta, a.vocab);
+  sl.per_warp = ((per_cta + kPickWarps - 1) / kPickWarps + 7) / 8 * 8;
+  const float temp = a.temperature[seq];
+  const bool greedy = !(temp > 0.f);
+  const double* u = a.uniforms + int64_t(seq) * (a.n_draft + 1);
+  const int32_t* drafts = a.drafts + int64_t(seq) * a.n_draft;
+  int32_t* out = a.tokens + int64_t(seq) * (a.n_draft + 1);
+  Weights<T> w;
+  w.table = table;
+  w.c = 1.4426950408889634074 / double(temp);
+  w.q = nullptr;
+  w.total = 1.0;
+  auto set_row = [&](int i, float m) {
+    w.l = static_cast<const T*>(a.logits) + seq * a.logits_seq + i * a.logits_tok;
+    w.m = double(m);
+  };
+  auto probs_row = [&](int i) { return a.draft_probs + seq * a.probs_seq + i * a.probs_tok; };
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // Rows of 16 positions at a time, one a warp, alike in every CTA of the cluster.
+  auto load_rows = [&](int i0) {
+    const int i = i0 + warp;
+    if (i <= a.n_draft) {
+      const float c = exponent_scale(temp);
       const VerifyPart* p = a.parts + (int64_t(seq) * (a.n_draft + 1) + i) * a.splits;
       VerifyPart v{};
       v.m = ninf();
       v.best = 0x7fffffff;
       if (lane < a.splits) v = p[lane];
+      Row r;
+      r.x = i < a.n_draft ? drafts[i] : -1;
+      r.there = r.x >= 0 && r.x < a.vocab;
+      set_row(i, 0.f);
+      const float lx = r.there ? to_f32(w.l[r.x]) : 0.f;
+      r.qx = r.there && a.draft_probs ? probs_row(i)[r.x] : 0.f;
       float m = v.m;
 #pragma unroll
       for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-      const double f = v.m == ninf() ? 0.0 : double(exp2f((v.m - m) * c));
+      const double f = v.m == ninf() ? 1.0 : double(ex2((v.m - m) * c));
       double s = v.s * f, b = v.b * f;
       int best = v.m == m ? v.best : 0x7fffffff;
 #pragma unroll
@@ -193,222 +395,102 @@ struct Pick {
         b += __shfl_xor_sync(~0u, b, d);
         best = min(best, __shfl_xor_sync(~0u, best, d));
       }
-      const bool bad = __any_sync(~0u, v.bad != 0);
-      if (lane == 0) *row_box = Row{m, s, b, best, !bad && m > ninf() && m < -ninf()};
+      r.m = m, r.s = s, r.b = b, r.best = best;
+      r.usable = m > ninf() && m < -ninf() && s == s;
+      w.m = double(m);
+      r.wx = r.there && r.usable ? w.plain(lx) : 0.0;
+      if (lane == 0) rows[warp] = r;
     }
     __syncthreads();
-    const Row r = *row_box;
-    __syncthreads();
-    return r;
-  }
-
-  // Every CTA's v, in rank order, into all[].
-  __device__ void exchange(double v, double (&all)[kMaxCluster]) {
-    if (threadIdx.x == 0) *box = v;
-    cl.sync();
-    for (unsigned r = 0; r < kMaxCluster; ++r) all[r] = r < cl.num_blocks() ? *cl.map_shared_rank(box, r) : 0.0;
-    cl.sync();
-  }
-};
-
-// The weight of element v of the drawn row: exp((l - m) / T), or what that over
-// the row's sum has above the draft's probability.
-template <typename T>
-struct Weights {
-  const T* l;
-  double m, t;
-  const float* q;      // nullptr: plain weights
-  double total;
-  __device__ __forceinline__ double plain(int v) const { return exp((double(to_f32(l[v])) - m) / t); }
-  __device__ __forceinline__ double operator()(int v) const {
-    const double w = plain(v);
-    if (!q) return w;
-    const double d = w / total - double(q[v]);
-    return d > 0.0 ? d : 0.0;
-  }
-};
-
-// This CTA's slice [lo, hi) of the vocabulary; its warps hold equal contiguous parts.
-struct Slice {
-  int lo, hi, per_warp;
-};
-
-template <typename T>
-__device__ double slice_sum(Pick& k, const Weights<T>& w, const Slice& sl, double& warp_part) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int b = min(sl.lo + warp * sl.per_warp, sl.hi), e = min(b + sl.per_warp, sl.hi);
-  double v = 0;
-#pragma unroll 4
-  for (int j = b + lane; j < e; j += 32) v += w(j);
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
-  warp_part = v;
-  if (lane == 0) k.warp_box[warp] = v;
-  __syncthreads();
-  double t = 0;
-  for (int x = 0; x < kPickWarps; ++x) t += k.warp_box[x];
-  return t;       // warp_box keeps the parts
-}
-
-// The lowest v whose running sum passes `goal`, by the whole cluster; sums is each
-// CTA's total and warp_box each warp's.  Where rounding leaves none, the last
-// element with a weight.
-template <typename T>
-__device__ int find(Pick& k, const Weights<T>& w, const Slice& sl, const double (&sums)[kMaxCluster], double goal) {
-  const unsigned n = k.cl.num_blocks(), me = k.cl.block_rank();
-  unsigned who = 0;
-  double before = 0, run = 0;
-  bool found = false;
-  for (unsigned r = 0; r < n && !found; ++r) {
-    if (sums[r] > 0) who = r, before = run;
-    run += sums[r];
-    found = run > goal;
-  }
-  if (me == who && threadIdx.x < 32) {
-    const int lane = threadIdx.x;
-    double base = before;
-    run = before;
-    int wp = 0;
-    found = false;
-    for (int x = 0; x < kPickWarps && !found; ++x) {
-      const double s = k.warp_box[x];
-      if (s > 0) wp = x, base = run;
-      run += s;
-      found = run > goal;
-    }
-    const int b = min(sl.lo + wp * sl.per_warp, sl.hi), e = min(b + sl.per_warp, sl.hi);
-    // a contiguous run of elements a lane
-    const int per = (e - b + 31) / 32;
-    const int lb = min(b + lane * per, e), le = min(lb + per, e);
-    double v = 0;
-    for (int j = lb; j < le; ++j) v += w(j);
-    double incl = v;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const double o = __shfl_up_sync(~0u, incl, d);
-      if (lane >= d) incl += o;
-    }
-    unsigned pass = __ballot_sync(~0u, v > 0 && base + incl > goal);
-    if (!pass) {
-      const unsigned any = __ballot_sync(~0u, v > 0);
-      pass = any ? 1u << (31 - __clz(any)) : 1u;
-    }
-    const int ln = __ffs(pass) - 1;
-    base += __shfl_sync(~0u, incl - v, ln);
-    // that lane's elements, one a lane
-    const int b2 = min(b + ln * per, e), e2 = min(b2 + per, e);
-    int token = -1, last = -1;
-    for (int j = b2; j < e2 && token < 0; j += 32) {
-      v = j + lane < e2 ? w(j + lane) : 0.0;
-      incl = v;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const double o = __shfl_up_sync(~0u, incl, d);
-        if (lane >= d) incl += o;
-      }
-      const unsigned hit = __ballot_sync(~0u, v > 0 && base + incl > goal), any = __ballot_sync(~0u, v > 0);
-      if (hit) token = j + __ffs(hit) - 1;
-      if (any) last = j + 31 - __clz(any);
-      base += __shfl_sync(~0u, incl, 31);
-    }
-    if (token < 0) token = last < 0 ? b2 : last;
-    if (lane == 0)
-      for (unsigned r = 0; r < n; ++r) *k.cl.map_shared_rank(k.int_box, r) = token;
-  }
-  k.cl.sync();
-  const int token = *k.int_box;
-  k.cl.sync();
-  return token;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const __grid_constant__ VerifyArgs a) {
-  __shared__ double box, warp_box[kPickWarps];
-  __shared__ int int_box;
-  __shared__ Row row_box;
-  cg::cluster_group cl = cg::this_cluster();
-  const int seq = blockIdx.x / cl.num_blocks();
-  Pick k{a, cl, seq, &box, warp_box, &int_box, &row_box};
-  const int per_cta = (a.vocab + int(cl.num_blocks()) - 1) / int(cl.num_blocks());
-  Slice sl;
-  sl.lo = min(int(cl.block_rank()) * per_cta, a.vocab);
-  sl.hi = min(sl.lo + per_cta, a.vocab);
-  sl.per_warp = (per_cta + kPickWarps - 1) / kPickWarps;
-  const float temp = a.temperature[seq];
-  const bool greedy = !(temp > 0.f);
-  const double* u = a.uniforms + int64_t(seq) * (a.n_draft + 1);
-  const int32_t* drafts = a.drafts + int64_t(seq) * a.n_draft;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-
-  auto weights = [&](int i, const Row& r) {
-    Weights<T> w;
-    w.l = static_cast<const T*>(a.logits) + seq * a.logits_seq + i * a.logits_tok;
-    w.m = double(r.m);
-    w.t = double(temp);
-    w.q = nullptr;
-    w.total = 1.0;
-    return w;
   };
-  double all[kMaxCluster], warp_part;
-  auto total_of = [&](const Weights<T>& w) {      // exact sum of the row; all[] and warp_box keep the parts
-    k.exchange(slice_sum(k, w, sl, warp_part), all);
+  double all[kMaxCluster];
+  int turn = 0;
+  auto total_of = [&]() {      // exact sum of w's row, by the cluster
+    const double mine = slice_sum(w, sl, box);
+    if (threadIdx.x == 0) box.sum[turn] = mine;
+    cl.sync();
     double t = 0;
-    for (unsigned r = 0; r < cl.num_blocks(); ++r) t += all[r];
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      all[r] = r < n_cta ? *cl.map_shared_rank(&box.sum[turn], r) : 0.0;
+      t += all[r];
+    }
+    turn ^= 1;
     return t;
   };
-  auto draw = [&](const Weights<T>& w, double at) {
-    const double t = total_of(w);
-    return find(k, w, sl, all, at * t);
-  };
 
-  int i = 0, token = -1;
+  int i = 0;
+  bool drawn = false;          // the last token comes from find
   bool usable = true;
+  int token = -1;
+  load_rows(0);
   for (;; ++i) {
-    const Row r = k.row(i);
+    if (i && i % kPickWarps == 0) {
+      __syncthreads();
+      load_rows(i);
+    }
+    const Row r = rows[i % kPickWarps];
     usable = r.usable;
-    const int x = i < a.n_draft ? drafts[i] : -1;
-    const bool there = x >= 0 && x < a.vocab;
     if (!usable) break;
     if (greedy) {
       token = r.best;
-      if (there && x == token) continue;
+      if (r.there && r.x == token) continue;
       break;
     }
-    const Weights<T> w = weights(i, r);
+    set_row(i, r.m);
+    w.q = nullptr;
+    w.wide = a.wide_logits;
     if (!a.draft_probs) {
-      if (there) {
-        const double goal = u[i] * r.s, wx = exp((double(to_f32(w.l[x])) - w.m) / w.t), edge = kOpen * r.s;
-        if (goal > r.b + edge && goal < r.b + wx - edge) continue;      // kept, whatever the rounding
-      }
-      token = draw(w, u[i]);
-      if (there && x == token) continue;
-      break;
-    }
-    const float* q = a.draft_probs + seq * a.probs_seq + i * a.probs_tok;
-    if (there) {
-      const double have = u[i] * double(q[x]) * r.s, wx = w.plain(x);
-      bool keep = have < wx;
-      if (!(fabs(have - wx) > kOpen * fmax(have, wx)) && have > 0.0) keep = u[i] * double(q[x]) < wx / total_of(w);
-      if (keep) continue;
-    }
-    Weights<T> wr = w;
-    const double goal = u[a.n_draft];
-    if (there) {
-      wr.q = q;
-      wr.total = total_of(w);
-      const double over = total_of(wr);
-      if (over > 0) {
-        token = find(k, wr, sl, all, goal * over);
+      const double goal = u[i] * r.s, edge = kOpen * r.s;
+      const bool in = goal > r.b + edge && goal < r.b + r.wx - edge;
+      const bool off = goal < r.b - edge || goal > r.b + r.wx + edge;
+      if (r.there && in) continue;                  // kept, whatever the rounding
+      const double t = total_of();
+      if (r.there && !off) {                        // open: the token drawn decides
+        find(w, sl, box, all, n_cta, me, u[i] * t, [&](int v) {
+          for (int k = 0; k < n_cta; ++k) *cl.map_shared_rank(&box.token, k) = v;
+        });
+        cl.sync();
+        token = box.token;
+        cl.sync();
+        if (token == r.x) continue;
         break;
       }
+      find(w, sl, box, all, n_cta, me, u[i] * t, [&](int v) { out[i] = v; });
+      drawn = true;
+      break;
     }
-    token = draw(w, goal);
+    double total = 0;
+    bool have_total = false;
+    if (r.there) {
+      const double want = u[i] * double(r.qx), have = want * r.s;
+      bool keep = have < r.wx;
+      if (!(fabs(have - r.wx) > kOpen * fmax(have, r.wx)) && have > 0.0) {
+        total = total_of();
+        have_total = true;
+        keep = want < r.wx / total;
+      }
+      if (keep) continue;
+    }
+    if (!have_total) total = total_of();
+    double sum = total;
+    if (r.there) {
+      w.q = probs_row(i);
+      w.total = total;
+      w.wide = a.wide_logits && a.wide_probs;
+      sum = total_of();
+      if (!(sum > 0)) {
+        w.q = nullptr;
+        sum = total_of();
+      }
+    }
+    find(w, sl, box, all, n_cta, me, u[a.n_draft] * sum, [&](int v) { out[i] = v; });
+    drawn = true;
     break;
   }
-  if (cl.block_rank() == 0) {
-    int32_t* out = a.tokens + int64_t(seq) * (a.n_draft + 1);
+  if (me == 0) {
     for (int j = threadIdx.x; j <= a.n_draft; j += kPickThreads)
-      out[j] = j < i ? drafts[j] : j == i && usable ? token : -1;
+      if (j != i || !drawn) out[j] = j < i ? drafts[j] : j == i && usable ? token : -1;
     if (threadIdx.x == 0) a.counts[seq] = i + (usable ? 1 : 0);
   }
   cl.sync();      // no CTA leaves while another may still read its shared memory
@@ -417,8 +499,14 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const __grid_
 template <typename T>
 cudaError_t launch_t(const VerifyArgs& args, int cluster, cudaStream_t s) {
   VerifyArgs a = args;
+  a.wide_logits = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.logits_seq * int64_t(sizeof(T)) % 16 == 0 &&
+                  a.logits_tok * int64_t(sizeof(T)) % 16 == 0;
+  a.wide_probs = reinterpret_cast<uintptr_t>(a.draft_probs) % 16 == 0 && a.probs_seq % 4 == 0 && a.probs_tok % 4 == 0;
   const dim3 grid(unsigned(a.n_seqs) * unsigned(a.n_draft + 1), unsigned(a.splits));
-  verify_stat_kernel<T><<<grid, kStatThreads, 0, s>>>(a);
+  if (a.draft_probs)
+    verify_stat_kernel<T, false><<<grid, kStatThreads, 0, s>>>(a);
+  else
+    verify_stat_kernel<T, true><<<grid, kStatThreads, 0, s>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
