@@ -1238,7 +1238,6 @@ vc_status vc_paged_attention(vc_ctx* c, const vc_kv_desc* d, int32_t layer, int3
   if (e != cudaSuccess) return fail(VC_ECUDA, "vc_paged_attention: %s", cudaGetErrorString(e));
   if (workspace_bytes < plan.workspace)
     return fail(VC_EINVAL, "vc_paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, plan.workspace);
-  a.n_workers = plan.n_workers;
   e = launch_paged_attn(a, plan, c->stream);
   if (e != cudaSuccess) return fail(VC_ECUDA, "vc_paged_attention launch: %s", cudaGetErrorString(e));
   return VC_OK;
@@ -1299,7 +1298,7 @@ vc_status vc_verify_tokens(vc_ctx* c, int32_t n_seqs, int32_t n_draft, int32_t v
   a.parts = static_cast<VerifyPart*>(workspace);
   a.tokens = tokens;
   a.counts = counts;
-  const cudaError_t e = launch_verify(a, logits_dtype, c->stream);
+  const cudaError_t e = launch_verify(a, logits_dtype, c->n_sm, c->stream);
   if (e != cudaSuccess) return fail(VC_ECUDA, "vc_verify_tokens launch: %s", cudaGetErrorString(e));
   return VC_OK;
 }

@@ -7,12 +7,14 @@
 // read once, for 4 * n_new * group operations per element (group = query heads
 // of one KV head), far under the tensor cores' rate for a few new tokens.
 //
-// Work split.  A unit is (sequence, KV head, tile of up to R query rows); its
-// rows' keys come in tiles of 64.  All units' tiles are laid end to end and cut
-// into equal contiguous ranges, one per worker CTA (a fixed number of CTAs that
-// are all resident), so a ragged batch and a single long sequence both spread
-// evenly without the host knowing the lengths.  A unit that one worker holds
-// whole is written by it; the others' parts (running maximum, sum and
+// Work split.  All sequences' keys, in tiles of 64, are laid end to end and cut
+// into equal contiguous ranges; a worker CTA takes one range for one unit (KV
+// head, tile of up to R query rows).  The number of ranges is set so that the
+// workers are all resident at once, so a ragged batch and a single long sequence
+// both spread evenly without the host knowing the lengths.  The units of a range
+// are neighbouring CTAs: they read the heads of the same cache rows, which lie
+// side by side in memory, at about the same time.  A sequence that lies in one
+// range is written by its worker; the others' parts (running maximum, sum and
 // unnormalised output, f32) go to the workspace and a second, dependent kernel
 // joins them.  Parts are joined in a fixed order, so results do not depend on
 // timing.
@@ -62,25 +64,25 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sum) {
   return v;
 }
 
-struct Place {        // where a worker's first tile lies
+struct Place {        // where a range's first tile lies
   int seq;
   int64_t seq_base;   // first tile of that sequence
   int64_t total;      // tiles in all
 };
 
-__device__ __forceinline__ int64_t chunk_of(int64_t total, int n_workers) {
-  return (total + n_workers - 1) / n_workers;
+__device__ __forceinline__ int64_t chunk_of(int64_t total, int n_ranges) {
+  return (total + n_ranges - 1) / n_ranges;
 }
 
-// The sequence that holds tile `worker * chunk`, found by the whole block.
-__device__ Place locate(const AttnArgs& a, int units, int worker) {
+// The sequence that holds tile `range * chunk`, found by the whole block.
+__device__ Place locate(const AttnArgs& a, int range) {
   __shared__ int64_t warp_sum[kWarps];
   __shared__ int64_t found_base, found_total;
   __shared__ int found_seq;
   int64_t v0 = 0, incl0 = 0, base = 0;
   for (int c = 0; c < a.n_seqs; c += kThreads) {
     const int s = c + threadIdx.x;
-    const int64_t v = s < a.n_seqs ? seq_tiles(a, s) * units : 0;
+    const int64_t v = s < a.n_seqs ? seq_tiles(a, s) : 0;
     const int64_t incl = base + block_scan(v, warp_sum);
     if (c == 0) v0 = v, incl0 = incl;
     if (threadIdx.x == kThreads - 1) found_total = incl;
@@ -88,7 +90,7 @@ __device__ Place locate(const AttnArgs& a, int units, int worker) {
     base = found_total;
   }
   const int64_t total = base;
-  const int64_t begin = int64_t(worker) * chunk_of(total, a.n_workers);
+  const int64_t begin = int64_t(range) * chunk_of(total, a.n_ranges);
   Place pl{0, 0, total};
   if (begin >= total) return pl;
   base = 0;
@@ -96,7 +98,7 @@ __device__ Place locate(const AttnArgs& a, int units, int worker) {
     int64_t v = v0, incl = incl0;
     if (c) {
       const int s = c + threadIdx.x;
-      v = s < a.n_seqs ? seq_tiles(a, s) * units : 0;
+      v = s < a.n_seqs ? seq_tiles(a, s) : 0;
       incl = base + block_scan(v, warp_sum);
     }
     if (incl - v <= begin && begin < incl) {
@@ -152,18 +154,28 @@ __device__ __forceinline__ RowAt row_at(const AttnArgs& a, int seq, int kvh, int
 // A part in the workspace: R rows of DP outputs, then R x (maximum, sum).
 template <int R, int DP> constexpr int64_t part_floats() { return int64_t(R) * DP + 2 * R; }
 
-// Shared memory of a unit's end: each warp's outputs, maxima (base-2 exponents) and sums.
+// Shared memory of a unit's end: each warp's outputs, maxima (base-2 exponents) and
+// sums, R rows at a time.  Rows are padded by 16 bytes: a warp's stores then fall
+// into different banks.
 template <int R, int DP>
 struct Merge {
-  float o[kWarps][R][DP];
+  float o[kWarps][R][DP + 4];
   float m[kWarps][R];
   float l[kWarps][R];
 };
 
-// The warps' results of one unit (or part of one), joined and written.
+// 2^x for x <= 0, within 2^-22 of itself; nothing below 2^-126.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The warps' results of R rows from row0, joined and written: the outputs, or a part
+// (whose rows are at `rows` and whose maxima and sums at `ml`).
 template <typename T, int R, int DP>
 __device__ __forceinline__ void emit(const AttnArgs& a, Merge<R, DP>& mg, int seq, int kvh, int row0, bool whole,
-                                     float* part) {
+                                     float* rows, float* ml) {
   __syncthreads();
   constexpr int kPer = R * DP / 4;     // float4 groups
   for (int i = threadIdx.x; i < kPer; i += kThreads) {
@@ -176,7 +188,7 @@ __device__ __forceinline__ void emit(const AttnArgs& a, Merge<R, DP>& mg, int se
     float l = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = exp2f(mg.m[w][r] - ref);
+      const float f = ex2(mg.m[w][r] - ref);
       l += f * mg.l[w][r];
       const float4 x = *reinterpret_cast<const float4*>(&mg.o[w][r][d]);
       o.x += f * x.x;
@@ -185,8 +197,8 @@ __device__ __forceinline__ void emit(const AttnArgs& a, Merge<R, DP>& mg, int se
       o.w += f * x.w;
     }
     if (!whole) {
-      *reinterpret_cast<float4*>(part + r * DP + d) = o;
-      if (d == 0) *reinterpret_cast<float2*>(part + R * DP + 2 * r) = make_float2(top, l);
+      *reinterpret_cast<float4*>(rows + r * DP + d) = o;
+      if (d == 0) *reinterpret_cast<float2*>(ml + 2 * r) = make_float2(top, l);
       continue;
     }
     if (row0 + r >= a.rows || d >= a.head_dim) continue;
@@ -238,279 +250,344 @@ template <> struct Bits<__half> {
   }
 };
 
-__device__ __forceinline__ uint4 ldg16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+
+// 16 bytes from global to shared memory without a register; zeros where size is 0.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int size) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
+}
+__device__ __forceinline__ void ldsm(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 
-// One warp's running state over the keys it is given, 16 at a time.  No shared
-// memory: K and V go from global memory straight into tensor-core fragments.
+// The sequence that holds a tile, and what a warp needs of it.
+struct Cursor {
+  int seq, len, nt;
+  int64_t base;       // its first tile
+  __device__ __forceinline__ void at(const AttnArgs& a, int s, int64_t b) {
+    seq = s, base = b;
+    len = int(seq_len(a, s));
+    nt = (len + kTile - 1) / kTile;
+  }
+  __device__ __forceinline__ void advance(const AttnArgs& a, int64_t tile) {
+    while (tile >= base + nt) at(a, seq + 1, base + nt);
+  }
+};
+
+// What one worker keeps in shared memory: a ring of stages a warp (16 keys' K rows,
+// then their V rows), then what the end of a unit needs; more query rows than
+// registers hold share that place while the unit runs.
+template <int R, int DP>
+struct TcShape {
+  static constexpr int kStage = 16 * DP * 2 * 2;
+  static constexpr int kStages = DP == 64 ? 6 : 3;      // 96 KB a CTA (DP = 256: 192 KB)
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr bool kQShared = R > 16;
+  static constexpr int kQRows = (R + 15) / 16 * 16;
+  static constexpr size_t kTail = kQShared && kQRows * DP * 2 > sizeof(Merge<8, DP>) ? kQRows * DP * 2 : sizeof(Merge<8, DP>);
+  static constexpr size_t kSmem = kRing + kTail;
+};
+
+// Attention of up to R query rows on the tensor cores, K and V rows of 16-bit types.
 //
-// Scores S = Q K^T (m16n8k16, rows = query rows, columns = keys).  The products'
-// inner index may be any order of the head's elements as long as Q and K agree,
-// so lane (n, c) = (lane / 4, lane % 4) takes the 16-byte chunks 4i + c of key
-// row n: its 8 elements are the B fragment of two inner steps, and the same
-// chunk of Q's row n is their A fragment.  With R = 8 the fragment's rows 8..15
-// are zeros.
+// What bounds it is how many bytes are on their way: 6.5 TB/s at some 2 us of loaded
+// latency needs 13 MB, 90 KB an SM.  Registers cannot hold that next to the
+// accumulators (a first version did, and read at 4.9 TB/s), so every warp has its own
+// ring of stages that cp.async fills two stages ahead, across sequence boundaries too;
+// no warp waits for another but at a unit's end.  A copy instruction covers whole
+// rows (half-line requests measured 17 % slower), rows are swizzled so that ldmatrix
+// reads without bank conflicts, and block-table entries are read one stage early.
 //
-// Outputs O^T = V^T P^T (rows = head elements, columns = query rows): the scores'
-// accumulators, rounded, are P^T's B fragment without any exchange.  V^T's A
-// fragment wants two keys' values of one element in a register: lane (r, c) loads
-// chunk 8e + r of keys 2c, 2c+1, 2c+8, 2c+9 and pairs them with byte permutes.
+// Scores S = Q K^T (rows = query rows, columns = keys).  Outputs O^T = V^T P^T (rows =
+// head elements, columns = query rows): the scores' accumulators, rounded, are P^T's
+// fragment without any exchange, and ldmatrix.trans gives V^T.
 //
 // P is rounded to 16 bits twice (its value, then what that left over), so the
-// products see 16 (bf16) or more bits of it; the row sums are taken in f32.  The
-// loop waits on memory, and the second product of 8 is free.
+// products see 16 (bf16) or more bits of it and the output keeps the error of its
+// own rounding; the row sums are taken in f32.
 template <typename T, int R, int DP>
-struct TensorCore {
-  static constexpr int kRows = R, kDP = DP;
-  static constexpr int KS = DP / 32;      // 16-byte chunks a lane holds of a K row
-  static constexpr int VS = DP / 64;      // ... and of each of its V rows
-  static constexpr int RT = R / 8;        // column tiles of P^T
+__global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_kernel(const __grid_constant__ AttnArgs a) {
   using B = Bits<T>;
+  using Shape = TcShape<R, DP>;
+  constexpr int KS = DP / 16;          // inner steps of Q K^T, row tiles of O^T
+  constexpr int MT = (R + 15) / 16;    // row tiles of S
+  constexpr int NT = R / 8;            // column tiles of P^T
+  constexpr int kStages = Shape::kStages;
+  constexpr int kCols = DP / 8;        // 16-byte chunks of a row
+  constexpr int kRowsPerCopy = 32 / kCols > 0 ? 32 / kCols : 1;
+  extern __shared__ __align__(128) char smem[];
+  Merge<8, DP>& mg = *reinterpret_cast<Merge<8, DP>*>(smem + Shape::kRing);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
+  const uint32_t ring = smem_addr(smem) + warp * (kStages * Shape::kStage);
+  const uint32_t qs = smem_addr(smem + Shape::kRing);
+  const int row_tiles = (a.rows + R - 1) / R;
+  const int units = a.n_kv_heads * row_tiles;
+  const int range = blockIdx.x / units, unit = blockIdx.x - range * units;
+  const int rt = unit / a.n_kv_heads, kvh = unit - rt * a.n_kv_heads, row0 = rt * R;
+  const int group = a.n_heads / a.n_kv_heads;
+  const Place pl = locate(a, range);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t chunk = chunk_of(pl.total, a.n_ranges);
+  const int64_t begin = int64_t(range) * chunk;
+  const int64_t end = begin + chunk < pl.total ? begin + chunk : pl.total;
+  if (begin >= end) return;
+  float* parts = a.parts + int64_t(blockIdx.x) * 2 * part_floats<R, DP>();
 
-  uint32_t q[RT][KS][4];
-  float o[RT][VS * 4][4];
-  float m[RT], l[RT];
-  int lim[RT];                 // rows seen: key < lim
-  uint4 kf[2][KS];             // K rows n and n + 8 of the tile to come
-  uint4 vf[4][VS];             // V rows of the four keys
-  int64_t off;                 // lane i < 16: row offset of key i of the loaded tile, -1: none
-
-  __device__ __forceinline__ void begin(const AttnArgs& a, int seq, int kvh, int row0, int len) {
-    const int lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const int r = row0 + t * 8 + n;
-      const bool real = r < a.rows;
-      const RowAt at = row_at(a, seq, kvh, real ? r : 0);
-      lim[t] = real ? len - a.n_new + 1 + at.tok : 0;
-      const T* src = static_cast<const T*>(a.q) + at.q;
-#pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        const int e = (i * 4 + c) * 8;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (real && e < a.head_dim) x = *reinterpret_cast<const uint4*>(src + e);
-        q[t][i][0] = x.x, q[t][i][1] = x.y, q[t][i][2] = x.z, q[t][i][3] = x.w;
+  // ---- loading: lane i < 16 finds key i's row, one stage before it is copied
+  Cursor ahead;
+  ahead.at(a, pl.seq, pl.seq_base);
+  int64_t next = begin;                // tile the registers below describe
+  int page = 0, slot = 0;
+  bool real = false;
+  auto look = [&]() {
+    real = false;
+    if (next < end) {
+      ahead.advance(a, next);
+      const int p = int(next - ahead.base) * kTile + warp * 16 + lane;
+      if (lane < 16 && p < ahead.len) {
+        const int block = unsigned(p) / unsigned(a.block_size);
+        page = __ldg(a.block_tables + int64_t(ahead.seq) * a.max_blocks + block);
+        slot = p - block * a.block_size;
+        real = true;
       }
+    }
+  };
+  int fill = 0;                        // stage to fill
+  auto issue = [&]() {
+    if (next < end) {
+      int64_t off = -1;
+      if (real) {
+        off = int64_t(page) * a.stride_page + int64_t(slot) * a.stride_row;
+        if (page < 0 || off + a.row_span > a.cache_elems) {
+          *a.err = 1;
+          off = -1;
+        } else {
+          off += kvh * a.stride_head;
+        }
+      }
+      ++next;
+      look();
+      const uint32_t dst = ring + fill * Shape::kStage;
+#pragma unroll
+      for (int j = 0; j < 16; j += kRowsPerCopy) {
+        const int row = j + (kCols < 32 ? lane / kCols : 0), col = lane % kCols;
+        const int64_t o = __shfl_sync(~0u, off, row);
+        const int size = o >= 0 && col * 8 < a.head_dim ? 16 : 0;
+        const int64_t at = size ? o + col * 8 : 0;
+        const uint32_t d = dst + row * (DP * 2) + ((col ^ (row & 7)) << 4);
+        copy16(d, static_cast<const T*>(a.k) + at, size);
+        copy16(d + 16 * DP * 2, static_cast<const T*>(a.v) + at, size);
+      }
+    }
+    fill = fill + 1 == kStages ? 0 : fill + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  look();
+  for (int i = 0; i < kStages - 1; ++i) issue();
+
+  // ---- one sequence's part of the range after the other
+  // lane's row and half of the four 8x8 blocks that a ldmatrix reads
+  const int key = ((lane >> 4) << 3) + (lane & 7), half = (lane >> 3) & 1, flip = lane & 7;
+  uint32_t q[Shape::kQShared ? 1 : KS][4];
+  float o[NT][KS][4];
+  float m[NT], l[NT];
+  int lim[NT];
+  int use = 0;                         // stage to use
+  Cursor now;
+  now.at(a, pl.seq, pl.seq_base);
+  int64_t cur = begin;
+  while (cur < end) {
+    now.advance(a, cur);
+    const int seq = now.seq, len = now.len;
+    const int t0 = int(cur - now.base);
+    const int t1 = now.nt - t0 < end - cur ? now.nt : t0 + int(end - cur);
+    // the query rows: fragments in registers, or rows in shared memory
+    if constexpr (Shape::kQShared) {
+      for (int i = threadIdx.x; i < Shape::kQRows * kCols; i += kThreads) {
+        const int r = i / kCols, col = i - r * kCols;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < R && row0 + r < a.rows && col * 8 < a.head_dim)
+          x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + row_at(a, seq, kvh, row0 + r).q + col * 8);
+        *reinterpret_cast<uint4*>(smem + Shape::kRing + r * (DP * 2) + ((col ^ (r & 7)) << 4)) = x;
+      }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = row0 + h * 8 + n;
+        const bool has = h * 8 < R && r < a.rows;
+        const T* src = static_cast<const T*>(a.q) + row_at(a, seq, kvh, has ? r : 0).q;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int e = ks * 16 + x * 8 + 2 * c;
+            q[ks][h + 2 * x] = has && e < a.head_dim ? *reinterpret_cast<const uint32_t*>(src + e) : 0u;
+          }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int r = row0 + t * 8 + n;
+      lim[t] = r < a.rows ? len - a.n_new + 1 + r / group : 0;
       m[t] = ninf();
       l[t] = 0.f;
 #pragma unroll
-      for (int i = 0; i < VS * 4; ++i)
+      for (int i = 0; i < KS; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[t][i][j] = 0.f;
     }
-  }
-
-  // Row offsets of the 16 keys from p0 (lane i < 16 holds key i's).
-  __device__ __forceinline__ void find(const AttnArgs& a, int seq, int kvh, int p0, int len) {
-    const int lane = threadIdx.x & 31;
-    off = -1;
-    if (lane < 16 && p0 + lane < len) {
-      off = row_of(a, seq, p0 + lane);
-      if (off >= 0) off += kvh * a.stride_head;
-    }
-  }
-
-  __device__ __forceinline__ void load_k(const AttnArgs& a) {
-    const int lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int64_t at = __shfl_sync(~0u, off, n + 8 * x);
-      const T* src = static_cast<const T*>(a.k) + at;
-#pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        const int e = (i * 4 + c) * 8;
-        kf[x][i] = make_uint4(0, 0, 0, 0);
-        if (at >= 0 && e < a.head_dim) kf[x][i] = ldg16(src + e);
-      }
-    }
-  }
-
-  __device__ __forceinline__ void load_v(const AttnArgs& a) {
-    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int64_t at = __shfl_sync(~0u, off, 2 * c + (x & 1) + (x >> 1) * 8);
-      const T* src = static_cast<const T*>(a.v) + at;
-#pragma unroll
-      for (int i = 0; i < VS; ++i) {
-        const int e = (i * 8 + r) * 8;
-        vf[x][i] = make_uint4(0, 0, 0, 0);
-        if (at >= 0 && e < a.head_dim) vf[x][i] = ldg16(src + e);
-      }
-    }
-  }
-
-  static __device__ __forceinline__ uint32_t word(const uint4& v, int f) {
-    return f == 0 ? v.x : f == 1 ? v.y : f == 2 ? v.z : v.w;
-  }
-
-  // acc += V^T P^T of the 16 keys for one column tile; key x of the lane's four dropped where `keep` says so.
-  __device__ __forceinline__ void pv(float (&acc)[VS * 4][4], const uint32_t (&hi)[2], const uint32_t (&lo)[2],
-                                     unsigned keep = 15u) {
-#pragma unroll
-    for (int i = 0; i < VS; ++i)
-#pragma unroll
-      for (int f = 0; f < 4; ++f) {
-        uint32_t w[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) w[x] = (keep >> x) & 1 ? word(vf[x][i], f) : 0u;
-        const uint32_t a0 = __byte_perm(w[0], w[1], 0x5410), a1 = __byte_perm(w[0], w[1], 0x7632);
-        const uint32_t a2 = __byte_perm(w[2], w[3], 0x5410), a3 = __byte_perm(w[2], w[3], 0x7632);
-        B::mma(acc[i * 4 + f], a0, a1, a2, a3, hi[0], hi[1]);
-        B::mma(acc[i * 4 + f], a0, a1, a2, a3, lo[0], lo[1]);
-      }
-  }
-
-  __device__ __forceinline__ bool wild() const {       // an infinity or NaN among the lane's V values
-    bool bad = false;
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-#pragma unroll
-      for (int i = 0; i < VS; ++i)
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          const uint32_t w = word(vf[x][i], f);
-          bad = bad || (w & B::kExp) == B::kExp || ((w >> 16) & B::kExp) == B::kExp;
-        }
-    return bad;
-  }
-
-  // The 16 keys from p0, whose K rows are in kf; next_k then issues the next loads of K.
-  template <typename NextK>
-  __device__ __forceinline__ void keys(const AttnArgs& a, int p0, int len, int row0, NextK next_k) {
-    const int lane = threadIdx.x & 31, c = lane & 3;
-    float s[RT][2][4];
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[t][x][j] = 0.f;
-    // with two column tiles, rows 8..15 of the fragment are the second one
-#pragma unroll
-    for (int i = 0; i < KS; ++i)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const uint32_t r1a = RT == 2 ? q[RT - 1][i][0] : 0u, r1b = RT == 2 ? q[RT - 1][i][1] : 0u;
-        const uint32_t r1c = RT == 2 ? q[RT - 1][i][2] : 0u, r1d = RT == 2 ? q[RT - 1][i][3] : 0u;
-        B::mma(s[0][x], q[0][i][0], r1a, q[0][i][1], r1b, kf[x][i].x, kf[x][i].y);
-        B::mma(s[0][x], q[0][i][2], r1c, q[0][i][3], r1d, kf[x][i].z, kf[x][i].w);
-      }
-    if constexpr (RT == 2) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) s[1][x][0] = s[0][x][2], s[1][x][1] = s[0][x][3];
-    }
-    next_k();
-    uint32_t hi[RT][2], lo[RT][2];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      float top = ninf();
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int p = p0 + 8 * x + 2 * c + j;
-          s[t][x][j] = p < lim[t] ? s[t][x][j] * a.scale_log2 : ninf();
-          top = fmaxf(top, s[t][x][j]);
-        }
-      top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-      top = fmaxf(top, m[t]);
-      if (__any_sync(~0u, top > m[t])) {
-        // the maximum grew: what is summed so far shrinks (rarely after the first tiles)
-        const float f = m[t] == ninf() ? 0.f : exp2f(m[t] - top);
-        l[t] *= f;
-        const float f0 = __shfl_sync(~0u, f, c * 8), f1 = __shfl_sync(~0u, f, c * 8 + 4);
-#pragma unroll
-        for (int i = 0; i < VS * 4; ++i) {
-          o[t][i][0] *= f0, o[t][i][2] *= f0;
-          o[t][i][1] *= f1, o[t][i][3] *= f1;
-        }
-        m[t] = top;
-      }
-      const float ref = m[t] == ninf() ? 0.f : m[t];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float e0 = exp2f(s[t][x][0] - ref), e1 = exp2f(s[t][x][1] - ref);
-        l[t] += e0 + e1;
-        hi[t][x] = B::pack(e0, e1);
-        const float2 h = B::unpack(hi[t][x]);
-        lo[t][x] = B::pack(e0 - h.x, e1 - h.y);
-      }
-    }
-    // Rows that differ in what they see share this tile: 0 * infinity of a value that
-    // only later tokens see must not reach an earlier token's row.
-    const bool mixed = p0 + 16 > len - a.n_new + 1 && a.n_new > 1;
-    if (mixed && __any_sync(~0u, wild())) {
-      const int group = a.n_heads / a.n_kv_heads;
 #pragma unroll 1
-      for (int tok = row0 / group; tok < a.n_new && tok * group < row0 + R; ++tok) {
-        unsigned keep = 0;
+    for (int p0 = t0 * kTile + warp * 16; p0 < t1 * kTile; p0 += kTile) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncwarp();                    // the stage has landed for all lanes, and the one before is free
+      issue();
+      const uint32_t kst = ring + use * Shape::kStage, vst = kst + 16 * DP * 2;
+      use = use + 1 == kStages ? 0 : use + 1;
+      float s[MT][2][4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          if (p0 + 2 * c + (x & 1) + (x >> 1) * 8 < len - a.n_new + 1 + tok) keep |= 1u << x;
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          float acc[VS * 4][4] = {};
-          pv(acc, hi[t], lo[t], keep);
-          const int r = row0 + t * 8 + 2 * c;
-          const bool c0 = r / group == tok, c1 = (r + 1) / group == tok;
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int i = 0; i < VS * 4; ++i) {
-            if (c0) o[t][i][0] += acc[i][0], o[t][i][2] += acc[i][2];
-            if (c1) o[t][i][1] += acc[i][1], o[t][i][3] += acc[i][3];
+          for (int j = 0; j < 4; ++j) s[i][x][j] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint32_t kf[4];
+        ldsm(kst + key * (DP * 2) + (((ks * 2 + half) ^ flip) << 4), kf);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          if constexpr (Shape::kQShared) {
+            // blocks of a Q fragment: rows 0-7 and 8-15 of the left half, then of the right
+            uint32_t qf[4];
+            const int qr = i * 16 + half * 8 + (lane & 7), qc = ks * 2 + (lane >> 4);
+            ldsm(qs + qr * (DP * 2) + ((qc ^ (qr & 7)) << 4), qf);
+            B::mma(s[i][0], qf[0], qf[1], qf[2], qf[3], kf[0], kf[1]);
+            B::mma(s[i][1], qf[0], qf[1], qf[2], qf[3], kf[2], kf[3]);
+          } else {
+            B::mma(s[i][0], q[ks][0], q[ks][1], q[ks][2], q[ks][3], kf[0], kf[1]);
+            B::mma(s[i][1], q[ks][0], q[ks][1], q[ks][2], q[ks][3], kf[2], kf[3]);
           }
         }
       }
-    } else {
+      const int sure = len - a.n_new + 1;        // every row sees the keys before it
+      const bool all_seen = p0 + 16 <= sure;
+      uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
-      for (int t = 0; t < RT; ++t) pv(o[t], hi[t], lo[t]);
-    }
-  }
-
-  // Tiles [t0, t1) of the unit: this warp's 16 keys of each.
-  __device__ __forceinline__ void run(const AttnArgs& a, int seq, int kvh, int row0, int len, int t0, int t1) {
-    const int warp = threadIdx.x >> 5;
-    int p0 = t0 * kTile + warp * 16;
-    find(a, seq, kvh, p0, len);
-    load_k(a);
-    load_v(a);
-    begin(a, seq, kvh, row0, len);
+      for (int t = 0; t < NT; ++t) {
+        float x[2][2], top = ninf();
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            x[i][j] = s[t / 2][i][(t & 1) * 2 + j] * a.scale_log2;
+            if (!all_seen && p0 + 8 * i + 2 * c + j >= lim[t]) x[i][j] = ninf();
+            top = fmaxf(top, x[i][j]);
+          }
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+        top = fmaxf(top, m[t]);
+        if (__any_sync(~0u, top > m[t])) {
+          // the maximum grew: what is summed so far shrinks (rarely after the first tiles)
+          const float f = m[t] == ninf() ? 0.f : ex2(m[t] - top);
+          l[t] *= f;
+          const float f0 = __shfl_sync(~0u, f, c * 8), f1 = __shfl_sync(~0u, f, c * 8 + 4);
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            o[t][i][0] *= f0, o[t][i][2] *= f0;
+            o[t][i][1] *= f1, o[t][i][3] *= f1;
+          }
+          m[t] = top;
+        }
+        const float ref = m[t] == ninf() ? 0.f : m[t];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float e0 = ex2(x[i][0] - ref), e1 = ex2(x[i][1] - ref);
+          l[t] += e0 + e1;
+          hi[t][i] = B::pack(e0, e1);
+          const float2 h = B::unpack(hi[t][i]);
+          lo[t][i] = B::pack(e0 - h.x, e1 - h.y);
+        }
+      }
+      const uint32_t vrow = vst + key * (DP * 2);
+      // Rows that see different keys share this tile: 0 * infinity of a value that only
+      // later tokens see must not reach an earlier token's row.
+      bool wild = false;
+      if (!all_seen && a.n_new > 1) {
 #pragma unroll 1
-    for (int t = t0; t < t1; ++t, p0 += kTile) {
-      const bool more = t + 1 < t1;
-      keys(a, p0, len, row0, [&] {
-        if (more) {
-          find(a, seq, kvh, p0 + kTile, len);
-          load_k(a);
+        for (int i = lane; i < 16 * kCols; i += 32) {
+          uint4 v;
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(vst + i * 16));
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          for (int j = 0; j < 4; ++j)
+            wild = wild || (w[j] & B::kExp) == B::kExp || ((w[j] >> 16) & B::kExp) == B::kExp;
         }
-      });
-      if (more) load_v(a);
-    }
-  }
-
-  __device__ __forceinline__ void store(Merge<R, DP>& mg) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
+        wild = __any_sync(~0u, wild);
+      }
+      if (!wild) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      l[t] += __shfl_xor_sync(~0u, l[t], 1);
-      l[t] += __shfl_xor_sync(~0u, l[t], 2);
-      if (c == 0) mg.m[warp][t * 8 + r] = m[t], mg.l[warp][t * 8 + r] = l[t];
+        for (int i = 0; i < KS; ++i) {
+          uint32_t vf[4];
+          ldsm_t(vrow + (((i * 2 + half) ^ flip) << 4), vf);
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < VS; ++i) {
-          float* dst = &mg.o[warp][t * 8 + 2 * c + j][(i * 8 + r) * 8];
-#pragma unroll
-          for (int f = 0; f < 4; ++f) dst[2 * f] = o[t][i * 4 + f][j], dst[2 * f + 1] = o[t][i * 4 + f][2 + j];
+          for (int t = 0; t < NT; ++t) {
+            B::mma(o[t][i], vf[0], vf[1], vf[2], vf[3], hi[t][0], hi[t][1]);
+            B::mma(o[t][i], vf[0], vf[1], vf[2], vf[3], lo[t][0], lo[t][1]);
+          }
         }
+      } else {
+        // token by token from the last: the rows that it does not see become zeros, and
+        // only its columns are kept
+#pragma unroll 1
+        for (int tok = min(a.n_new, (row0 + R + group - 1) / group) - 1; tok >= row0 / group; --tok) {
+#pragma unroll 1
+          for (int i = lane; i < 16 * kCols; i += 32)
+            if (p0 + i / kCols >= sure + tok)
+              asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(vst + i * 16), "r"(0) : "memory");
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            uint32_t vf[4];
+            ldsm_t(vrow + (((i * 2 + half) ^ flip) << 4), vf);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              const int r = row0 + t * 8 + 2 * c;
+              const bool c0 = r / group == tok, c1 = (r + 1) / group == tok;
+              float y[4] = {o[t][i][0], o[t][i][1], o[t][i][2], o[t][i][3]};
+              B::mma(y, vf[0], vf[1], vf[2], vf[3], hi[t][0], hi[t][1]);
+              B::mma(y, vf[0], vf[1], vf[2], vf[3], lo[t][0], lo[t][1]);
+              if (c0) o[t][i][0] = y[0], o[t][i][2] = y[2];
+              if (c1) o[t][i][1] = y[1], o[t][i][3] = y[3];
+            }
+          }
+          __syncwarp();
+        }
+      }
     }
+    // the four warps' results, eight rows at a time; a part that begins its sequence
+    // goes to slot 1, one that continues it to slot 0
+    const bool whole = t0 == 0 && t1 == now.nt;
+    float* part = parts + (t0 == 0 ? part_floats<R, DP>() : 0);
+    if constexpr (Shape::kQShared) __syncthreads();      // the query rows make place
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float sum = l[t] + __shfl_xor_sync(~0u, l[t], 1);
+      sum += __shfl_xor_sync(~0u, sum, 2);
+      if (c == 0) mg.m[warp][n] = m[t], mg.l[warp][n] = sum;
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mg.o[warp][2 * c + (j & 1)][i * 16 + (j >> 1) * 8 + n] = o[t][i][j];
+      emit<T, 8, DP>(a, mg, seq, kvh, row0 + t * 8, whole, part + t * 8 * DP, part + R * DP + t * 16);
+    }
+    cur += t1 - t0;
   }
-};
+}
 
 // ---------------------------- f32 rows, and 16-bit rows of any alignment: FMAs
 
@@ -546,7 +623,7 @@ struct Fma {
   }
 
   __device__ __forceinline__ void run(const AttnArgs& a, int seq, int kvh, int row0, int len, int t0, int t1,
-                                      float (*qs)[DP]) {
+                                      float (*qs)[DP + 4]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane & 7;
     for (int i = threadIdx.x; i < R * DP; i += kThreads) {
       const int r = i / DP, d = i - r * DP;
@@ -638,48 +715,46 @@ struct Fma {
 
 // ------------------------------------------------------------------ kernels
 
-template <typename T, typename Core, bool kFma>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_constant__ AttnArgs a) {
+template <typename T, typename Core>
+__global__ void __launch_bounds__(kThreads) paged_attn_fma_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int R = Core::kRows, DP = Core::kDP;
-  extern __shared__ __align__(16) char smem[];
+  extern __shared__ __align__(128) char smem[];
   Merge<R, DP>& mg = *reinterpret_cast<Merge<R, DP>*>(smem);
   const int row_tiles = (a.rows + R - 1) / R;
   const int units = a.n_kv_heads * row_tiles;
-  const Place pl = locate(a, units, blockIdx.x);
+  const int range = blockIdx.x / units, unit = blockIdx.x - range * units;
+  const int rt = unit / a.n_kv_heads, kvh = unit - rt * a.n_kv_heads, row0 = rt * R;
+  const Place pl = locate(a, range);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t chunk = chunk_of(pl.total, a.n_workers);
-  int64_t cur = int64_t(blockIdx.x) * chunk;
+  const int64_t chunk = chunk_of(pl.total, a.n_ranges);
+  int64_t cur = int64_t(range) * chunk;
   const int64_t end = cur + chunk < pl.total ? cur + chunk : pl.total;
   int seq = pl.seq;
   int64_t base = pl.seq_base;
   float* parts = a.parts + int64_t(blockIdx.x) * 2 * part_floats<R, DP>();
   while (cur < end) {
     const int64_t nt = seq_tiles(a, seq);
-    if (cur >= base + nt * units) {
-      base += nt * units;
+    if (cur >= base + nt) {
+      base += nt;
       ++seq;
       continue;
     }
-    const int unit = int((cur - base) / nt);
-    const int t0 = int((cur - base) - unit * nt);
+    const int t0 = int(cur - base);
     const int t1 = nt - t0 < end - cur ? int(nt) : t0 + int(end - cur);
-    const int kvh = unit / row_tiles, row0 = (unit - kvh * row_tiles) * R;
     const int len = int(seq_len(a, seq));
     Core core;
-    if constexpr (kFma)
-      core.run(a, seq, kvh, row0, len, t0, t1, mg.o[0]);      // the queries sit where the outputs will
-    else
-      core.run(a, seq, kvh, row0, len, t0, t1);
-    if constexpr (kFma) __syncthreads();
+    core.run(a, seq, kvh, row0, len, t0, t1, mg.o[0]);      // the queries sit where the outputs will
+    __syncthreads();
     core.store(mg);
-    // a part that begins its unit goes to slot 1, one that continues a unit to slot 0
-    emit<T, R, DP>(a, mg, seq, kvh, row0, t0 == 0 && t1 == nt, parts + (t0 == 0 ? part_floats<R, DP>() : 0));
+    // a part that begins its sequence goes to slot 1, one that continues it to slot 0
+    float* part = parts + (t0 == 0 ? part_floats<R, DP>() : 0);
+    emit<T, R, DP>(a, mg, seq, kvh, row0, t0 == 0 && t1 == nt, part, part + R * DP);
     cur += t1 - t0;
   }
 }
 
-// One query row: the parts of its unit joined in worker order; units that one
-// worker held whole are done, units without a key get zeros.
+// One query row: the parts of its sequence joined in the ranges' order; sequences
+// in one range are done, those without a key get zeros.
 template <typename T, int R, int DP>
 __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __grid_constant__ AttnArgs a) {
   __shared__ int64_t warp_sum[kWarps];
@@ -693,7 +768,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __g
   // tiles before this sequence, and in all
   int64_t before = 0, total = 0;
   for (int s = threadIdx.x; s < a.n_seqs; s += kJoinThreads) {
-    const int64_t v = seq_tiles(a, s) * units;
+    const int64_t v = seq_tiles(a, s);
     total += v;
     if (s < seq) before += v;
   }
@@ -719,13 +794,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __g
   // every CTA waits for the first kernel, so that what follows this one does too
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (nt == 0) return;
-  const int64_t chunk = chunk_of(total, a.n_workers);
-  const int64_t first = before + int64_t(kvh * row_tiles + row / R) * nt;
-  const int64_t wa = first / chunk, wb = (first + nt - 1) / chunk;
+  const int64_t chunk = chunk_of(total, a.n_ranges);
+  const int64_t wa = before / chunk, wb = (before + nt - 1) / chunk;
   if (wa == wb) return;
   const int r = row % R;
   constexpr int64_t kPart = part_floats<R, DP>();
-  auto part = [&](int64_t w) { return a.parts + (w * 2 + (w == wa ? 1 : 0)) * kPart; };
+  const int unit = row / R * a.n_kv_heads + kvh;
+  auto part = [&](int64_t w) { return a.parts + ((w * units + unit) * 2 + (w == wa ? 1 : 0)) * kPart; };
   float top = ninf();
   for (int64_t w = wa + threadIdx.x; w <= wb; w += kJoinThreads) top = fmaxf(top, __ldcg(part(w) + R * DP + 2 * r));
 #pragma unroll
@@ -771,32 +846,37 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __g
 struct Variant {
   const void* main;
   const void* join;
-  int rows, dp;
+  int rows;
   size_t smem, part;
 };
 
-template <typename T, typename Core, bool kFma>
-Variant variant() {
-  constexpr int R = Core::kRows, DP = Core::kDP;
-  return {reinterpret_cast<const void*>(&paged_attn_kernel<T, Core, kFma>),
-          reinterpret_cast<const void*>(&paged_attn_join_kernel<T, R, DP>), R, DP, sizeof(Merge<R, DP>),
+template <typename T, int R, int DP>
+Variant tc() {
+  return {reinterpret_cast<const void*>(&paged_attn_tc_kernel<T, R, DP>),
+          reinterpret_cast<const void*>(&paged_attn_join_kernel<T, R, DP>), R, TcShape<R, DP>::kSmem,
           size_t(part_floats<R, DP>()) * sizeof(float)};
 }
 
-constexpr int kVariants = 18;
+template <typename T, int V, int DP>
+Variant fma_rows() {
+  using Core = Fma<T, V, DP>;
+  return {reinterpret_cast<const void*>(&paged_attn_fma_kernel<T, Core>),
+          reinterpret_cast<const void*>(&paged_attn_join_kernel<T, Core::kRows, DP>), Core::kRows,
+          sizeof(Merge<Core::kRows, DP>), size_t(part_floats<Core::kRows, DP>()) * sizeof(float)};
+}
+
+// [bf16, f16] x [8, 16, 40 query rows] x [64, 128, 256 elements] (40 rows of 256 do not
+// fit the registers), then f32 and the 16-bit types of any alignment.
+constexpr int kVariants = 24;
 const Variant& variant_at(int i) {
   using bf = __nv_bfloat16;
   using hf = __half;
   static const Variant v[kVariants] = {
-      variant<bf, TensorCore<bf, 8, 64>, false>(),  variant<bf, TensorCore<bf, 8, 128>, false>(),
-      variant<bf, TensorCore<bf, 8, 256>, false>(), variant<bf, TensorCore<bf, 16, 64>, false>(),
-      variant<bf, TensorCore<bf, 16, 128>, false>(), variant<hf, TensorCore<hf, 8, 64>, false>(),
-      variant<hf, TensorCore<hf, 8, 128>, false>(), variant<hf, TensorCore<hf, 8, 256>, false>(),
-      variant<hf, TensorCore<hf, 16, 64>, false>(), variant<hf, TensorCore<hf, 16, 128>, false>(),
-      variant<float, Fma<float, 4, 128>, true>(),   variant<float, Fma<float, 4, 256>, true>(),
-      variant<float, Fma<float, 1, 128>, true>(),   variant<float, Fma<float, 1, 256>, true>(),
-      variant<bf, Fma<bf, 1, 128>, true>(),         variant<bf, Fma<bf, 1, 256>, true>(),
-      variant<hf, Fma<hf, 1, 128>, true>(),         variant<hf, Fma<hf, 1, 256>, true>(),
+      tc<bf, 8, 64>(),  tc<bf, 8, 128>(),  tc<bf, 8, 256>(),  tc<bf, 16, 64>(), tc<bf, 16, 128>(), tc<bf, 16, 256>(),
+      tc<bf, 40, 64>(), tc<bf, 40, 128>(), tc<hf, 8, 64>(),   tc<hf, 8, 128>(), tc<hf, 8, 256>(),  tc<hf, 16, 64>(),
+      tc<hf, 16, 128>(), tc<hf, 16, 256>(), tc<hf, 40, 64>(), tc<hf, 40, 128>(),
+      fma_rows<float, 4, 128>(), fma_rows<float, 4, 256>(), fma_rows<float, 1, 128>(), fma_rows<float, 1, 256>(),
+      fma_rows<bf, 1, 128>(),    fma_rows<bf, 1, 256>(),    fma_rows<hf, 1, 128>(),    fma_rows<hf, 1, 256>(),
   };
   return v[i];
 }
@@ -805,7 +885,7 @@ const Variant& variant_at(int i) {
 
 namespace {
 
-cudaError_t plan_variant(int v, int n_sm, AttnPlan* plan) {
+cudaError_t plan_variant(int v, int n_kv_heads, int rows, int n_sm, AttnPlan* plan) {
   const Variant& k = variant_at(v);
   static int resident[kVariants];      // CTAs an SM holds; the same on every B200
   int n = __atomic_load_n(&resident[v], __ATOMIC_RELAXED);
@@ -818,8 +898,16 @@ cudaError_t plan_variant(int v, int n_sm, AttnPlan* plan) {
     if (n < 1) return cudaErrorInvalidConfiguration;
     __atomic_store_n(&resident[v], n, __ATOMIC_RELAXED);
   }
+  // Ranges: the workers just fill the GPU; where a range has so many units that this
+  // would leave a fifth of it idle, at least four rounds of workers.
+  const int64_t units = int64_t(n_kv_heads) * ((rows + k.rows - 1) / k.rows);
+  const int64_t slots = int64_t(n) * n_sm;
+  int64_t ranges = slots / units;
+  if (ranges * units * 5 < slots * 4 || ranges < 1) ranges = (4 * slots + units - 1) / units;
+  if (ranges * units > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
   plan->variant = v;
-  plan->n_workers = n * n_sm;
+  plan->n_ranges = int(ranges);
+  plan->n_workers = int(ranges * units);
   plan->workspace = size_t(plan->n_workers) * 2 * k.part;
   return cudaSuccess;
 }
@@ -828,9 +916,10 @@ cudaError_t plan_variant(int v, int n_sm, AttnPlan* plan) {
 int variant_for(const AttnArgs& a, int dtype, bool wide) {
   if (dtype != 1 && wide) {
     const int size = a.head_dim <= 64 ? 0 : a.head_dim <= 128 ? 1 : 2;
-    return (dtype == 0 ? 0 : 5) + (a.rows > 8 && size < 2 ? 3 + size : size);
+    const int tile = a.rows <= 8 ? 0 : a.rows <= 16 || size == 2 ? 1 : 2;
+    return (dtype == 0 ? 0 : 8) + tile * 3 + size;
   }
-  return (dtype == 1 ? (wide ? 10 : 12) : dtype == 0 ? 14 : 16) + (a.head_dim <= 128 ? 0 : 1);
+  return (dtype == 1 ? (wide ? 16 : 18) : dtype == 0 ? 20 : 22) + (a.head_dim <= 128 ? 0 : 1);
 }
 
 }  // namespace
@@ -839,7 +928,7 @@ cudaError_t paged_attn_workspace(const AttnArgs& a, int dtype, int n_sm, size_t*
   *bytes = 0;
   for (int wide = 0; wide < 2; ++wide) {
     AttnPlan p;
-    const cudaError_t e = plan_variant(variant_for(a, dtype, wide != 0), n_sm, &p);
+    const cudaError_t e = plan_variant(variant_for(a, dtype, wide != 0), a.n_kv_heads, a.rows, n_sm, &p);
     if (e != cudaSuccess) return e;
     if (p.workspace > *bytes) *bytes = p.workspace;
   }
@@ -853,7 +942,7 @@ cudaError_t plan_paged_attn(const AttnArgs& a, int dtype, int n_sm, AttnPlan* pl
   bool wide = true;
   for (int64_t s : strides) wide = wide && s * esz % 16 == 0;
   for (const void* p : ptrs) wide = wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
-  return plan_variant(variant_for(a, dtype, wide), n_sm, plan);
+  return plan_variant(variant_for(a, dtype, wide), a.n_kv_heads, a.rows, n_sm, plan);
 }
 
 cudaError_t launch_paged_attn(const AttnArgs& args, const AttnPlan& plan, cudaStream_t s) {
@@ -861,7 +950,8 @@ cudaError_t launch_paged_attn(const AttnArgs& args, const AttnPlan& plan, cudaSt
   AttnArgs a = args;
   void* params[] = {&a};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(a.n_workers));
+  cfg.gridDim = dim3(unsigned(plan.n_workers));
+  a.n_ranges = plan.n_ranges;
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = k.smem;
   cfg.stream = s;

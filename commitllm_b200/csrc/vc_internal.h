@@ -193,12 +193,13 @@ struct AttnArgs {
   void* out;                   // [n_seqs][n_new][n_heads][head_dim]
   float* lse;                  // [n_seqs][n_new][n_heads] or nullptr
   float* parts;                // partial results of split units
-  int32_t n_workers;
+  int32_t n_ranges;            // ranges of keys
   int* err;
 };
 struct AttnPlan {
   int variant;                 // index of the kernel
-  int n_workers;               // CTAs
+  int n_ranges;
+  int n_workers;               // CTAs: ranges x units
   size_t workspace;            // bytes of parts
 };
 cudaError_t paged_attn_workspace(const AttnArgs& a, int dtype, int n_sm, size_t* bytes);
@@ -225,7 +226,7 @@ struct VerifyArgs {
   int32_t* counts;             // [n_seqs]
 };
 void plan_verify(VerifyArgs* a, int n_sm);
-cudaError_t launch_verify(const VerifyArgs& a, int dtype, cudaStream_t s);
+cudaError_t launch_verify(const VerifyArgs& a, int dtype, int n_sm, cudaStream_t s);
 
 // int_peak.cu
 cudaError_t launch_int_peak(int variant, int64_t iters, int n_sm, uint32_t* sink, cudaStream_t s,

@@ -93,22 +93,13 @@ struct Running {
   }
 };
 
-template <typename T, bool kBefore>
-__global__ void __launch_bounds__(kStatThreads) verify_stat_kernel(const __grid_constant__ VerifyArgs a) {
+template <typename T, typename R>
+__device__ __forceinline__ void stat_slice(const T* src, int lo, int hi, float c, int x, R& r) {
   constexpr int N = 16 / sizeof(T);
   constexpr int kBatch = 4;           // 16-byte loads a thread has under way
   struct alignas(16) Chunk {
     T v[N];
   };
-  const int row = blockIdx.x, split = blockIdx.y;
-  const int seq = row / (a.n_draft + 1), i = row - seq * (a.n_draft + 1);
-  const T* src = static_cast<const T*>(a.logits) + seq * a.logits_seq + i * a.logits_tok;
-  const int lo = split * a.slice;
-  const int hi = min(lo + a.slice, a.vocab);
-  const float c = exponent_scale(a.temperature[seq]);
-  // without draft probabilities the part of the sum before the draft is wanted
-  const int x = kBefore && i < a.n_draft ? a.drafts[int64_t(seq) * a.n_draft + i] : -1;
-  Running<kBefore> r;
   // single elements up to the first 16-byte boundary, chunks, single elements
   const int head = lo < hi ? min(int((16 - (reinterpret_cast<uintptr_t>(src + lo) & 15)) & 15) / int(sizeof(T)), hi - lo) : 0;
   const int body = lo < hi ? (hi - lo - head) / N : 0;
@@ -139,6 +130,29 @@ __global__ void __launch_bounds__(kStatThreads) verify_stat_kernel(const __grid_
   if (tail + int(threadIdx.x) < hi) {
     const float l[1] = {to_f32(src[tail + threadIdx.x])};
     r.template add<1, 1>(l, tail + threadIdx.x, 0, c, x);
+  }
+}
+
+template <typename T, bool kBefore>
+__global__ void __launch_bounds__(kStatThreads) verify_stat_kernel(const __grid_constant__ VerifyArgs a) {
+  const int row = blockIdx.x, split = blockIdx.y;
+  const int seq = row / (a.n_draft + 1), i = row - seq * (a.n_draft + 1);
+  const T* src = static_cast<const T*>(a.logits) + seq * a.logits_seq + i * a.logits_tok;
+  const int lo = split * a.slice;
+  const int hi = min(lo + a.slice, a.vocab);
+  const float c = exponent_scale(a.temperature[seq]);
+  // without draft probabilities the part of the sum before the draft is wanted
+  const int x = kBefore && i < a.n_draft ? a.drafts[int64_t(seq) * a.n_draft + i] : -1;
+  // a slice behind x has none of that part, one before x all of it: only the slice
+  // that holds x looks at each element
+  Running<true> r;
+  if (kBefore && lo < x && x < hi) {
+    stat_slice<T>(src, lo, hi, c, x, r);
+  } else {
+    Running<false> rr;
+    stat_slice<T>(src, lo, hi, c, x, rr);
+    r.m = rr.m, r.s = rr.s, r.best = rr.best;
+    r.b = kBefore && x >= hi ? rr.s : 0.f;
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // the block's
@@ -176,24 +190,22 @@ __global__ void __launch_bounds__(kStatThreads) verify_stat_kernel(const __grid_
   }
 }
 
-// 2^t in f64 for t <= 0: 2^(j / 64) from a table (shared memory, made by exp2), the
-// rest |r| <= 1 / 128 by the series of 2^r up to r^5 (what follows is below 2^-54).
-// 11 f64 operations, about half of exp(): f64 arithmetic bounds the drawn row.
-constexpr int kTable = 64;
-__device__ __forceinline__ double pow2(double t, const double* table) {
-  if (t < -1000.0) return exp2(t);          // where results lose bits or vanish
+// 2^(y / 1024) in f64 for y in [-2^31, 0], 2^-1000 or so below that: 2^(j / 1024) from a table (shared memory,
+// made by exp2), the rest |r| <= 1/2 by the series of 2^(r / 1024) up to r^3 (what
+// follows is below 2^-50).  Seven f64 operations and no branch: f64 arithmetic bounds
+// the drawn row, and exp() takes about twenty.
+constexpr int kTable = 1024;
+__device__ __forceinline__ double pow2(double y, const double* table) {
   constexpr double kMagic = 6755399441055744.0;      // 1.5 * 2^52: rounds to a whole number
-  const double z = fma(t, double(kTable), kMagic);
+  const double z = y + kMagic;
   const int n = __double2loint(z);
-  const double r = fma(z - kMagic, -1.0 / kTable, t);
-  constexpr double l = 0.693147180559945309417;      // ln 2
-  double p = fma(r, l * l * l * l * l / 120, l * l * l * l / 24);
-  p = fma(r, p, l * l * l / 6);
-  p = fma(r, p, l * l / 2);
+  const double r = y - (z - kMagic);
+  constexpr double l = 0.693147180559945309417 / kTable;      // ln 2 / 1024
+  double p = fma(r, l * l * l / 6, l * l / 2);
   p = fma(r, p, l);
   const double v = table[n & (kTable - 1)];
   p = fma(r * p, v, v);
-  return __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p));
+  return __hiloint2double(__double2hiint(p) + (max(n >> 10, -1000) << 20), __double2loint(p));
 }
 
 // One position: its row's joined sums, and the draft's weight and probability.
@@ -212,13 +224,19 @@ struct Weights {
   const T* l;
   const float* q;      // nullptr: plain weights
   const double* table;
-  double m, c, total;
+  double m, c, scale;  // maximum, 1024 log2(e) / T, 1 / the row's sum
+  float none;          // logits below it weigh nothing: exp would round to 0
   bool wide;           // rows on 16-byte boundaries
-  __device__ __forceinline__ double plain(float x) const { return pow2((double(x) - m) * c, table); }
+  // (a weight from there to 2^-1000 counts as about 2^-1000: enough to be drawn at
+  // u = 0, nothing in a sum)
+  __device__ __forceinline__ double plain(float x) const {
+    const double w = pow2((double(x) - m) * c, table);
+    return x < none ? 0.0 : w;
+  }
   __device__ __forceinline__ double of(float x, float qv) const {
     const double w = plain(x);
     if (!q) return w;
-    const double d = w / total - double(qv);
+    const double d = fma(w, scale, -double(qv));
     return d > 0.0 ? d : 0.0;
   }
   __device__ __forceinline__ double at(int v) const { return of(to_f32(l[v]), q ? q[v] : 0.f); }
@@ -250,7 +268,7 @@ __device__ double slice_sum(const Weights<T>& w, const Slice& sl, Box& box) {
   int j = b;
   if (w.wide) {
     const int n = (e - b) / N;
-#pragma unroll 4
+#pragma unroll (16 / N)
     for (int k = lane; k < n; k += 32) {
       const Chunk ch = *reinterpret_cast<const Chunk*>(w.l + b + k * N);
       float qv[N] = {};
@@ -343,7 +361,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const __gr
   const int n_cta = int(cl.num_blocks()), me = int(cl.block_rank());
   const int seq = blockIdx.x / n_cta;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x < kTable) table[threadIdx.x] = exp2(double(threadIdx.x) / kTable);
+  for (int i = threadIdx.x; i < kTable; i += kPickThreads) table[i] = exp2(double(i) / kTable);
   Slice sl;
   const int per_cta = ((a.vocab + n_cta - 1) / n_cta + 7) / 8 * 8;
   sl.lo = min(me * per_cta, a.vocab);
@@ -356,12 +374,13 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const __gr
   int32_t* out = a.tokens + int64_t(seq) * (a.n_draft + 1);
   Weights<T> w;
   w.table = table;
-  w.c = 1.4426950408889634074 / double(temp);
+  w.c = kTable * 1.4426950408889634074 / double(temp);
   w.q = nullptr;
-  w.total = 1.0;
+  w.scale = 1.0;
   auto set_row = [&](int i, float m) {
     w.l = static_cast<const T*>(a.logits) + seq * a.logits_seq + i * a.logits_tok;
     w.m = double(m);
+    w.none = fmaxf(__fadd_ru(m, __fmul_rn(temp, -744.44f)), -3.4e38f);
   };
   auto probs_row = [&](int i) { return a.draft_probs + seq * a.probs_seq + i * a.probs_tok; };
   __syncthreads();
@@ -380,8 +399,8 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const __gr
       Row r;
       r.x = i < a.n_draft ? drafts[i] : -1;
       r.there = r.x >= 0 && r.x < a.vocab;
-      set_row(i, 0.f);
-      const float lx = r.there ? to_f32(w.l[r.x]) : 0.f;
+      const T* l = static_cast<const T*>(a.logits) + seq * a.logits_seq + i * a.logits_tok;
+      const float lx = r.there ? to_f32(l[r.x]) : 0.f;
       r.qx = r.there && a.draft_probs ? probs_row(i)[r.x] : 0.f;
       float m = v.m;
 #pragma unroll
@@ -397,7 +416,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const __gr
       }
       r.m = m, r.s = s, r.b = b, r.best = best;
       r.usable = m > ninf() && m < -ninf() && s == s;
-      w.m = double(m);
+      set_row(i, m);
       r.wx = r.there && r.usable ? w.plain(lx) : 0.0;
       if (lane == 0) rows[warp] = r;
     }
@@ -476,7 +495,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const __gr
     double sum = total;
     if (r.there) {
       w.q = probs_row(i);
-      w.total = total;
+      w.scale = 1.0 / total;
       w.wide = a.wide_logits && a.wide_probs;
       sum = total_of();
       if (!(sum > 0)) {
@@ -545,8 +564,11 @@ void plan_verify(VerifyArgs* a, int n_sm) {
   a->splits = int32_t((int64_t(a->vocab) + slice - 1) / slice);
 }
 
-cudaError_t launch_verify(const VerifyArgs& a, int dtype, cudaStream_t s) {
-  const int cluster = a.vocab > 4096 ? kMaxCluster : 1;
+cudaError_t launch_verify(const VerifyArgs& a, int dtype, int n_sm, cudaStream_t s) {
+  // CTAs of a sequence's cluster: as many as stay resident at once (two an SM), one
+  // for a short row
+  int cluster = a.vocab > 4096 ? kMaxCluster : 1;
+  while (cluster > 1 && int64_t(a.n_seqs) * cluster > 2 * n_sm) cluster /= 2;
   switch (dtype) {
     case 0: return launch_t<__nv_bfloat16>(a, cluster, s);
     case 1: return launch_t<float>(a, cluster, s);

@@ -230,6 +230,18 @@ def test_verify_extreme_temperatures(ctx):
     check(ctx, logits, drafts, u, t)
 
 
+@pytest.mark.parametrize("t", [1e-9, 1.03e-8, 1.1e-8, 1e-7, 1e-5])
+def test_verify_neighbouring_logits_at_small_temperatures(ctx, t):
+    """Logits one f32 step apart, where a step is from a fraction of the temperature to hundreds of it."""
+    V = 5000
+    l = np.full((8, 1, V), 100.0, np.float32)
+    step = np.nextafter(np.float32(100), np.float32(0)) - np.float32(100)
+    l[:, 0] += step * np.random.default_rng(19).integers(0, 4, (8, V)).astype(np.float32)
+    l[:, 0, 17:2000] -= 1
+    u = np.linspace(0, 0.999, 8)[:, None] + 1e-5 * np.pi
+    check(ctx, torch.tensor(l, device="cuda"), np.zeros((8, 0), np.int32), u, np.full(8, t, np.float32))
+
+
 def test_verify_is_captured_and_replayed(ctx):
     stream = torch.cuda.Stream()
     c2 = C.Context(0, stream)
