@@ -48,7 +48,8 @@ __device__ __forceinline__ int64_t seq_tiles(const AttnArgs& a, int s) {
   return (seq_len(a, s) + kTile - 1) / kTile;
 }
 
-// Inclusive sum of v over the block's 128 threads.
+// Inclusive sum of v over the block's W warps.
+template <int W>
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sum) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -59,7 +60,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sum) {
   if (lane == 31) warp_sum[warp] = v;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w)
+  for (int w = 0; w < W; ++w)
     if (w < warp) v += warp_sum[w];
   return v;
 }
@@ -75,17 +76,18 @@ __device__ __forceinline__ int64_t chunk_of(int64_t total, int n_ranges) {
 }
 
 // The sequence that holds tile `range * chunk`, found by the whole block.
+template <int W>
 __device__ Place locate(const AttnArgs& a, int range) {
-  __shared__ int64_t warp_sum[kWarps];
+  __shared__ int64_t warp_sum[W];
   __shared__ int64_t found_base, found_total;
   __shared__ int found_seq;
   int64_t v0 = 0, incl0 = 0, base = 0;
-  for (int c = 0; c < a.n_seqs; c += kThreads) {
+  for (int c = 0; c < a.n_seqs; c += (W * 32)) {
     const int s = c + threadIdx.x;
     const int64_t v = s < a.n_seqs ? seq_tiles(a, s) : 0;
-    const int64_t incl = base + block_scan(v, warp_sum);
+    const int64_t incl = base + block_scan<W>(v, warp_sum);
     if (c == 0) v0 = v, incl0 = incl;
-    if (threadIdx.x == kThreads - 1) found_total = incl;
+    if (threadIdx.x == (W * 32) - 1) found_total = incl;
     __syncthreads();
     base = found_total;
   }
@@ -94,19 +96,19 @@ __device__ Place locate(const AttnArgs& a, int range) {
   Place pl{0, 0, total};
   if (begin >= total) return pl;
   base = 0;
-  for (int c = 0; c < a.n_seqs; c += kThreads) {
+  for (int c = 0; c < a.n_seqs; c += (W * 32)) {
     int64_t v = v0, incl = incl0;
     if (c) {
       const int s = c + threadIdx.x;
       v = s < a.n_seqs ? seq_tiles(a, s) : 0;
-      incl = base + block_scan(v, warp_sum);
+      incl = base + block_scan<W>(v, warp_sum);
     }
     if (incl - v <= begin && begin < incl) {
       found_seq = c + threadIdx.x;
       found_base = incl - v;
     }
-    if (c + kThreads < a.n_seqs) {
-      if (threadIdx.x == kThreads - 1) found_total = incl;
+    if (c + (W * 32) < a.n_seqs) {
+      if (threadIdx.x == (W * 32) - 1) found_total = incl;
       __syncthreads();
       base = found_total;
       __syncthreads();
@@ -228,7 +230,7 @@ template <> struct Bits<__nv_bfloat16> {
   }
   static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
@@ -244,7 +246,7 @@ template <> struct Bits<__half> {
   }
   static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
@@ -280,18 +282,91 @@ struct Cursor {
 };
 
 // What one worker keeps in shared memory: a ring of stages a warp (16 keys' K rows,
-// then their V rows), then what the end of a unit needs; more query rows than
-// registers hold share that place while the unit runs.
+// then their V rows), then what the end of a unit needs.
 template <int R, int DP>
 struct TcShape {
   static constexpr int kStage = 16 * DP * 2 * 2;
   static constexpr int kStages = DP == 64 ? 6 : 3;      // 96 KB a CTA (DP = 256: 192 KB)
   static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr bool kQShared = R > 16;
-  static constexpr int kQRows = (R + 15) / 16 * 16;
-  static constexpr size_t kTail = kQShared && kQRows * DP * 2 > sizeof(Merge<8, DP>) ? kQRows * DP * 2 : sizeof(Merge<8, DP>);
-  static constexpr size_t kSmem = kRing + kTail;
+  static constexpr size_t kSmem = kRing + sizeof(Merge<8, DP>);
 };
+
+// Whether n 16-byte chunks of shared memory hold an infinity or a NaN (by the whole warp).
+template <typename B>
+__device__ __forceinline__ bool not_finite(uint32_t addr, int n) {
+  bool bad = false;
+#pragma unroll 1
+  for (int i = threadIdx.x & 31; i < n; i += 32) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr + i * 16));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    for (int j = 0; j < 4; ++j) bad = bad || (w[j] & B::kExp) == B::kExp || ((w[j] >> 16) & B::kExp) == B::kExp;
+  }
+  return __any_sync(~0u, bad);
+}
+
+// The halves of a V^T register (keys p and p + 1) that a row which sees keys below lim keeps.
+__device__ __forceinline__ uint32_t seen_pair(int p, int lim) {
+  return (p < lim ? 0xFFFFu : 0u) | (p + 1 < lim ? 0xFFFF0000u : 0u);
+}
+
+// o += V^T P^T in the columns (query rows) that belong to one token.
+template <typename B>
+__device__ __forceinline__ void pv_of_token(float (&o)[4], const uint32_t (&vf)[4], const uint32_t (&hi)[2],
+                                            const uint32_t (&lo)[2], bool c0, bool c1) {
+  float y[4] = {o[0], o[1], o[2], o[3]};
+  B::mma(y, vf[0], vf[1], vf[2], vf[3], hi[0], hi[1]);
+  B::mma(y, vf[0], vf[1], vf[2], vf[3], lo[0], lo[1]);
+  if (c0) o[0] = y[0], o[2] = y[2];
+  if (c1) o[1] = y[1], o[3] = y[3];
+}
+
+// Weights are taken relative to a reference that is at most 2^8 below the largest one
+// seen: it follows the maximum only when that has grown by more, so the sums so far are
+// seldom rescaled (a maximum of random scores grows in half of the first 30 tiles) and
+// no weight passes 2^8, which f16 holds too.
+constexpr float kSlack = 8.f;
+
+// Scores to weights for one column tile of 8 query rows (the lane's: lane / 4) and 16 keys
+// (the lane's: 2c, 2c + 1, 2c + 8, 2c + 9; those from `left` after 2c on are not seen):
+// the running reference and sum, the sums so far where the reference moves, and the
+// weights in two 16-bit parts.
+template <typename B, int KS>
+__device__ __forceinline__ void weigh(const float (&s)[2][2], float scale, int left, int c, float& m, float& l,
+                                      float (&o)[KS][4], uint32_t (&hi)[2], uint32_t (&lo)[2]) {
+  float x[2][2], top = ninf();
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      x[i][j] = 8 * i + j < left ? s[i][j] * scale : ninf();
+      top = fmaxf(top, x[i][j]);
+    }
+  top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+  if (__any_sync(~0u, top > m + kSlack)) {
+    // what is summed so far shrinks to the new maximum
+    top = fmaxf(top, m);
+    const float f = m == ninf() ? 0.f : ex2(m - top);
+    l *= f;
+    const float f0 = __shfl_sync(~0u, f, c * 8), f1 = __shfl_sync(~0u, f, c * 8 + 4);
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      o[i][0] *= f0, o[i][2] *= f0;
+      o[i][1] *= f1, o[i][3] *= f1;
+    }
+    m = top;
+  }
+  const float ref = m == ninf() ? 0.f : m;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float e0 = ex2(x[i][0] - ref), e1 = ex2(x[i][1] - ref);
+    l += e0 + e1;
+    hi[i] = B::pack(e0, e1);
+    const float2 h = B::unpack(hi[i]);
+    lo[i] = B::pack(e0 - h.x, e1 - h.y);
+  }
+}
 
 // Attention of up to R query rows on the tensor cores, K and V rows of 16-bit types.
 //
@@ -315,7 +390,6 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
   using B = Bits<T>;
   using Shape = TcShape<R, DP>;
   constexpr int KS = DP / 16;          // inner steps of Q K^T, row tiles of O^T
-  constexpr int MT = (R + 15) / 16;    // row tiles of S
   constexpr int NT = R / 8;            // column tiles of P^T
   constexpr int kStages = Shape::kStages;
   constexpr int kCols = DP / 8;        // 16-byte chunks of a row
@@ -324,13 +398,12 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
   Merge<8, DP>& mg = *reinterpret_cast<Merge<8, DP>*>(smem + Shape::kRing);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
   const uint32_t ring = smem_addr(smem) + warp * (kStages * Shape::kStage);
-  const uint32_t qs = smem_addr(smem + Shape::kRing);
   const int row_tiles = (a.rows + R - 1) / R;
   const int units = a.n_kv_heads * row_tiles;
   const int range = blockIdx.x / units, unit = blockIdx.x - range * units;
   const int rt = unit / a.n_kv_heads, kvh = unit - rt * a.n_kv_heads, row0 = rt * R;
   const int group = a.n_heads / a.n_kv_heads;
-  const Place pl = locate(a, range);
+  const Place pl = locate<kWarps>(a, range);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t chunk = chunk_of(pl.total, a.n_ranges);
   const int64_t begin = int64_t(range) * chunk;
@@ -393,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
   // ---- one sequence's part of the range after the other
   // lane's row and half of the four 8x8 blocks that a ldmatrix reads
   const int key = ((lane >> 4) << 3) + (lane & 7), half = (lane >> 3) & 1, flip = lane & 7;
-  uint32_t q[Shape::kQShared ? 1 : KS][4];
+  uint32_t q[KS][4];
   float o[NT][KS][4];
   float m[NT], l[NT];
   int lim[NT];
@@ -406,17 +479,6 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
     const int seq = now.seq, len = now.len;
     const int t0 = int(cur - now.base);
     const int t1 = now.nt - t0 < end - cur ? now.nt : t0 + int(end - cur);
-    // the query rows: fragments in registers, or rows in shared memory
-    if constexpr (Shape::kQShared) {
-      for (int i = threadIdx.x; i < Shape::kQRows * kCols; i += kThreads) {
-        const int r = i / kCols, col = i - r * kCols;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < R && row0 + r < a.rows && col * 8 < a.head_dim)
-          x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + row_at(a, seq, kvh, row0 + r).q + col * 8);
-        *reinterpret_cast<uint4*>(smem + Shape::kRing + r * (DP * 2) + ((col ^ (r & 7)) << 4)) = x;
-      }
-      __syncthreads();
-    } else {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = row0 + h * 8 + n;
@@ -430,7 +492,6 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
             q[ks][h + 2 * x] = has && e < a.head_dim ? *reinterpret_cast<const uint32_t*>(src + e) : 0u;
           }
       }
-    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int r = row0 + t * 8 + n;
@@ -449,123 +510,57 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
       issue();
       const uint32_t kst = ring + use * Shape::kStage, vst = kst + 16 * DP * 2;
       use = use + 1 == kStages ? 0 : use + 1;
-      float s[MT][2][4];
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[i][x][j] = 0.f;
+      float s[2][4] = {};
+      // fragments are read one step ahead of the products that use them
+      uint32_t kf[2][4];
+      ldsm(kst + key * (DP * 2) + ((half ^ flip) << 4), kf[0]);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        uint32_t kf[4];
-        ldsm(kst + key * (DP * 2) + (((ks * 2 + half) ^ flip) << 4), kf);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          if constexpr (Shape::kQShared) {
-            // blocks of a Q fragment: rows 0-7 and 8-15 of the left half, then of the right
-            uint32_t qf[4];
-            const int qr = i * 16 + half * 8 + (lane & 7), qc = ks * 2 + (lane >> 4);
-            ldsm(qs + qr * (DP * 2) + ((qc ^ (qr & 7)) << 4), qf);
-            B::mma(s[i][0], qf[0], qf[1], qf[2], qf[3], kf[0], kf[1]);
-            B::mma(s[i][1], qf[0], qf[1], qf[2], qf[3], kf[2], kf[3]);
-          } else {
-            B::mma(s[i][0], q[ks][0], q[ks][1], q[ks][2], q[ks][3], kf[0], kf[1]);
-            B::mma(s[i][1], q[ks][0], q[ks][1], q[ks][2], q[ks][3], kf[2], kf[3]);
-          }
-        }
+        if (ks + 1 < KS) ldsm(kst + key * (DP * 2) + ((((ks + 1) * 2 + half) ^ flip) << 4), kf[(ks + 1) & 1]);
+        const uint32_t(&k)[4] = kf[ks & 1];
+        B::mma(s[0], q[ks][0], q[ks][1], q[ks][2], q[ks][3], k[0], k[1]);
+        B::mma(s[1], q[ks][0], q[ks][1], q[ks][2], q[ks][3], k[2], k[3]);
       }
       const int sure = len - a.n_new + 1;        // every row sees the keys before it
       const bool all_seen = p0 + 16 <= sure;
       uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        float x[2][2], top = ninf();
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            x[i][j] = s[t / 2][i][(t & 1) * 2 + j] * a.scale_log2;
-            if (!all_seen && p0 + 8 * i + 2 * c + j >= lim[t]) x[i][j] = ninf();
-            top = fmaxf(top, x[i][j]);
-          }
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-        top = fmaxf(top, m[t]);
-        if (__any_sync(~0u, top > m[t])) {
-          // the maximum grew: what is summed so far shrinks (rarely after the first tiles)
-          const float f = m[t] == ninf() ? 0.f : ex2(m[t] - top);
-          l[t] *= f;
-          const float f0 = __shfl_sync(~0u, f, c * 8), f1 = __shfl_sync(~0u, f, c * 8 + 4);
-#pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            o[t][i][0] *= f0, o[t][i][2] *= f0;
-            o[t][i][1] *= f1, o[t][i][3] *= f1;
-          }
-          m[t] = top;
-        }
-        const float ref = m[t] == ninf() ? 0.f : m[t];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float e0 = ex2(x[i][0] - ref), e1 = ex2(x[i][1] - ref);
-          l[t] += e0 + e1;
-          hi[t][i] = B::pack(e0, e1);
-          const float2 h = B::unpack(hi[t][i]);
-          lo[t][i] = B::pack(e0 - h.x, e1 - h.y);
-        }
+        const float x[2][2] = {{s[0][t * 2], s[0][t * 2 + 1]}, {s[1][t * 2], s[1][t * 2 + 1]}};
+        weigh<B, KS>(x, a.scale_log2, all_seen ? 0x7fffffff : lim[t] - p0 - 2 * c, c, m[t], l[t], o[t], hi[t], lo[t]);
       }
       const uint32_t vrow = vst + key * (DP * 2);
       // Rows that see different keys share this tile: 0 * infinity of a value that only
       // later tokens see must not reach an earlier token's row.
-      bool wild = false;
-      if (!all_seen && a.n_new > 1) {
-#pragma unroll 1
-        for (int i = lane; i < 16 * kCols; i += 32) {
-          uint4 v;
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(vst + i * 16));
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          for (int j = 0; j < 4; ++j)
-            wild = wild || (w[j] & B::kExp) == B::kExp || ((w[j] >> 16) & B::kExp) == B::kExp;
-        }
-        wild = __any_sync(~0u, wild);
-      }
+      const bool wild = !all_seen && a.n_new > 1 && not_finite<B>(vst, 16 * kCols);
       if (!wild) {
+        uint32_t vf[2][4];
+        ldsm_t(vrow + ((half ^ flip) << 4), vf[0]);
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
-          uint32_t vf[4];
-          ldsm_t(vrow + (((i * 2 + half) ^ flip) << 4), vf);
+          if (i + 1 < KS) ldsm_t(vrow + ((((i + 1) * 2 + half) ^ flip) << 4), vf[(i + 1) & 1]);
+          const uint32_t(&v)[4] = vf[i & 1];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            B::mma(o[t][i], vf[0], vf[1], vf[2], vf[3], hi[t][0], hi[t][1]);
-            B::mma(o[t][i], vf[0], vf[1], vf[2], vf[3], lo[t][0], lo[t][1]);
-          }
+          for (int t = 0; t < NT; ++t) B::mma(o[t][i], v[0], v[1], v[2], v[3], hi[t][0], hi[t][1]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) B::mma(o[t][i], v[0], v[1], v[2], v[3], lo[t][0], lo[t][1]);
         }
       } else {
-        // token by token from the last: the rows that it does not see become zeros, and
-        // only its columns are kept
+        // token by token: keys that it does not see become zeros, and only its columns are kept
 #pragma unroll 1
-        for (int tok = min(a.n_new, (row0 + R + group - 1) / group) - 1; tok >= row0 / group; --tok) {
-#pragma unroll 1
-          for (int i = lane; i < 16 * kCols; i += 32)
-            if (p0 + i / kCols >= sure + tok)
-              asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(vst + i * 16), "r"(0) : "memory");
-          __syncwarp();
+        for (int tok = row0 / group; tok < a.n_new && tok * group < row0 + R; ++tok) {
+          const uint32_t m0 = seen_pair(p0 + 2 * c, sure + tok), m1 = seen_pair(p0 + 2 * c + 8, sure + tok);
 #pragma unroll
           for (int i = 0; i < KS; ++i) {
             uint32_t vf[4];
             ldsm_t(vrow + (((i * 2 + half) ^ flip) << 4), vf);
+            vf[0] &= m0, vf[1] &= m0, vf[2] &= m1, vf[3] &= m1;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               const int r = row0 + t * 8 + 2 * c;
-              const bool c0 = r / group == tok, c1 = (r + 1) / group == tok;
-              float y[4] = {o[t][i][0], o[t][i][1], o[t][i][2], o[t][i][3]};
-              B::mma(y, vf[0], vf[1], vf[2], vf[3], hi[t][0], hi[t][1]);
-              B::mma(y, vf[0], vf[1], vf[2], vf[3], lo[t][0], lo[t][1]);
-              if (c0) o[t][i][0] = y[0], o[t][i][2] = y[2];
-              if (c1) o[t][i][1] = y[1], o[t][i][3] = y[3];
+              pv_of_token<B>(o[t][i], vf, hi[t], lo[t], r / group == tok, (r + 1) / group == tok);
             }
           }
-          __syncwarp();
         }
       }
     }
@@ -573,7 +568,6 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
     // goes to slot 1, one that continues it to slot 0
     const bool whole = t0 == 0 && t1 == now.nt;
     float* part = parts + (t0 == 0 ? part_floats<R, DP>() : 0);
-    if constexpr (Shape::kQShared) __syncthreads();      // the query rows make place
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       float sum = l[t] + __shfl_xor_sync(~0u, l[t], 1);
@@ -584,6 +578,263 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
 #pragma unroll
         for (int j = 0; j < 4; ++j) mg.o[warp][2 * c + (j & 1)][i * 16 + (j >> 1) * 8 + n] = o[t][i][j];
       emit<T, 8, DP>(a, mg, seq, kvh, row0 + t * 8, whole, part + t * 8 * DP, part + R * DP + t * 16);
+    }
+    cur += t1 - t0;
+  }
+}
+
+// More than 16 query rows (drafted tokens): the CTA's warps share each stage of 64 keys.
+// WR row tiles of 16 query rows times two halves of the keys, one warp each; a warp
+// that held all rows would need 255 registers and leave two warps a scheduler, whose
+// dependent instructions then bound the loop (measured: 5.5 cycles an instruction, 72
+// us for attend of 35 rows where the bytes take 26).  With 48 rows a CTA, three warps a
+// scheduler and 92 B/clk of shared memory reads at the HBM's rate, of 128.
+template <int WR, int DP>
+struct RowsShape {
+  static constexpr int kWarpsHere = WR * 2;
+  static constexpr int kStage = kTile * DP * 2 * 2;
+  static constexpr int kStages = DP == 64 ? 6 : 3;
+  static constexpr int kRing = kStages * kStage;             // 96 KB
+  // a key half's results of 8 rows, as its lanes hold them: outputs, maximum, sum
+  static constexpr int kGive = (DP / 16 * 4 + 2) * 32 * 4;
+  static constexpr size_t kSmem = kRing + WR * kGive;
+};
+
+template <typename T, int WR, int DP>
+__global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __grid_constant__ AttnArgs a) {
+  using B = Bits<T>;
+  using Shape = RowsShape<WR, DP>;
+  constexpr int R = WR * 16;
+  constexpr int KS = DP / 16;
+  constexpr int kStages = Shape::kStages, kW = Shape::kWarpsHere;
+  constexpr int kCols = DP / 8;                        // 16-byte chunks of a row
+  constexpr int kRowsPerCopy = 32 / kCols;
+  constexpr int kCopies = (kTile / kRowsPerCopy + kW - 1) / kW;      // a warp's, of K and of V
+  extern __shared__ __align__(128) char smem[];
+  float* give = reinterpret_cast<float*>(smem + Shape::kRing);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
+  const int wr = warp >> 1, kh = warp & 1;
+  const uint32_t ring = smem_addr(smem);
+  const int row_tiles = (a.rows + R - 1) / R;
+  const int units = a.n_kv_heads * row_tiles;
+  const int range = blockIdx.x / units, unit = blockIdx.x - range * units;
+  const int rt = unit / a.n_kv_heads, kvh = unit - rt * a.n_kv_heads;
+  const int row0 = rt * R, wrow0 = row0 + wr * 16;
+  const int group = a.n_heads / a.n_kv_heads;
+  const Place pl = locate<kW>(a, range);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t chunk = chunk_of(pl.total, a.n_ranges);
+  const int64_t begin = int64_t(range) * chunk;
+  const int64_t end = begin + chunk < pl.total ? begin + chunk : pl.total;
+  if (begin >= end) return;
+  float* parts = a.parts + int64_t(blockIdx.x) * 2 * part_floats<R, DP>();
+
+  // ---- loading: a warp copies every kW-th group of kRowsPerCopy rows; lane i finds the i-th of its rows
+  Cursor ahead;
+  ahead.at(a, pl.seq, pl.seq_base);
+  int64_t next = begin;
+  int page = 0, slot = 0;
+  bool real = false;
+  const int my_group = warp + lane / kRowsPerCopy * kW, my_row = my_group * kRowsPerCopy + lane % kRowsPerCopy;
+  auto look = [&]() {
+    real = false;
+    if (next < end) {
+      ahead.advance(a, next);
+      const int p = int(next - ahead.base) * kTile + my_row;
+      if (lane < kCopies * kRowsPerCopy && my_row < kTile && p < ahead.len) {
+        const int block = unsigned(p) / unsigned(a.block_size);
+        page = __ldg(a.block_tables + int64_t(ahead.seq) * a.max_blocks + block);
+        slot = p - block * a.block_size;
+        real = true;
+      }
+    }
+  };
+  int fill = 0;
+  auto issue = [&]() {
+    if (next < end) {
+      int64_t off = -1;
+      if (real) {
+        off = int64_t(page) * a.stride_page + int64_t(slot) * a.stride_row;
+        if (page < 0 || off + a.row_span > a.cache_elems) {
+          *a.err = 1;
+          off = -1;
+        } else {
+          off += kvh * a.stride_head;
+        }
+      }
+      ++next;
+      look();
+      const uint32_t dst = ring + fill * Shape::kStage;
+#pragma unroll
+      for (int j = 0; j < kCopies; ++j) {
+        const int row = (warp + j * kW) * kRowsPerCopy + lane / kCols, col = lane % kCols;
+        const int64_t o = __shfl_sync(~0u, off, j * kRowsPerCopy + lane / kCols);
+        if (row < kTile) {
+          const int size = o >= 0 && col * 8 < a.head_dim ? 16 : 0;
+          const int64_t at = size ? o + col * 8 : 0;
+          const uint32_t d = dst + row * (DP * 2) + ((col ^ (row & 7)) << 4);
+          copy16(d, static_cast<const T*>(a.k) + at, size);
+          copy16(d + kTile * DP * 2, static_cast<const T*>(a.v) + at, size);
+        }
+      }
+    }
+    fill = fill + 1 == kStages ? 0 : fill + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  look();
+  for (int i = 0; i < kStages - 1; ++i) issue();
+
+  const int key = ((lane >> 4) << 3) + (lane & 7), half = (lane >> 3) & 1, flip = lane & 7;
+  uint32_t q[KS][4];
+  float o[2][KS][4];
+  float m[2], l[2];
+  int lim[2];
+  int use = 0;
+  Cursor now;
+  now.at(a, pl.seq, pl.seq_base);
+  int64_t cur = begin;
+  while (cur < end) {
+    now.advance(a, cur);
+    const int seq = now.seq, len = now.len;
+    const int t0 = int(cur - now.base);
+    const int t1 = now.nt - t0 < end - cur ? now.nt : t0 + int(end - cur);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = wrow0 + h * 8 + n;
+      const bool has = r < a.rows;
+      const T* src = static_cast<const T*>(a.q) + row_at(a, seq, kvh, has ? r : 0).q;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int e = ks * 16 + x * 8 + 2 * c;
+          q[ks][h + 2 * x] = has && e < a.head_dim ? *reinterpret_cast<const uint32_t*>(src + e) : 0u;
+        }
+      lim[h] = has ? len - a.n_new + 1 + r / group : 0;
+      m[h] = ninf();
+      l[h] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[h][i][j] = 0.f;
+    }
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncthreads();                 // the stage has landed for all warps, and the one before is free
+      issue();
+      const uint32_t kst = ring + use * Shape::kStage, vst = kst + kTile * DP * 2;
+      use = use + 1 == kStages ? 0 : use + 1;
+      const int sure = len - a.n_new + 1;
+#pragma unroll 1
+      for (int b = 0; b < 2; ++b) {
+        const int at = kh * 32 + b * 16;               // rows of the stage
+        const int p0 = t * kTile + at;
+        const uint32_t krow = kst + (at + key) * (DP * 2), vrow = vst + (at + key) * (DP * 2);
+        float s[2][4] = {};
+        uint32_t kf[2][4];
+        ldsm(krow + ((half ^ flip) << 4), kf[0]);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          if (ks + 1 < KS) ldsm(krow + ((((ks + 1) * 2 + half) ^ flip) << 4), kf[(ks + 1) & 1]);
+          const uint32_t(&k)[4] = kf[ks & 1];
+          B::mma(s[0], q[ks][0], q[ks][1], q[ks][2], q[ks][3], k[0], k[1]);
+          B::mma(s[1], q[ks][0], q[ks][1], q[ks][2], q[ks][3], k[2], k[3]);
+        }
+        const bool all_seen = p0 + 16 <= sure;
+        uint32_t hi[2][2], lo[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float x[2][2] = {{s[0][h * 2], s[0][h * 2 + 1]}, {s[1][h * 2], s[1][h * 2 + 1]}};
+          weigh<B, KS>(x, a.scale_log2, all_seen ? 0x7fffffff : lim[h] - p0 - 2 * c, c, m[h], l[h], o[h], hi[h], lo[h]);
+        }
+        // rows that see different keys share this tile: see paged_attn_tc_kernel
+        const bool wild = !all_seen && a.n_new > 1 && not_finite<B>(vst + at * (DP * 2), 16 * kCols);
+        if (!wild) {
+          uint32_t vf[2][4];
+          ldsm_t(vrow + ((half ^ flip) << 4), vf[0]);
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            if (i + 1 < KS) ldsm_t(vrow + ((((i + 1) * 2 + half) ^ flip) << 4), vf[(i + 1) & 1]);
+            const uint32_t(&v)[4] = vf[i & 1];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) B::mma(o[h][i], v[0], v[1], v[2], v[3], hi[h][0], hi[h][1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) B::mma(o[h][i], v[0], v[1], v[2], v[3], lo[h][0], lo[h][1]);
+          }
+        } else {
+#pragma unroll 1
+          for (int tok = wrow0 / group; tok < a.n_new && tok * group < wrow0 + 16; ++tok) {
+            const uint32_t m0 = seen_pair(p0 + 2 * c, sure + tok), m1 = seen_pair(p0 + 2 * c + 8, sure + tok);
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+              uint32_t vf[4];
+              ldsm_t(vrow + (((i * 2 + half) ^ flip) << 4), vf);
+              vf[0] &= m0, vf[1] &= m0, vf[2] &= m1, vf[3] &= m1;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int r = wrow0 + h * 8 + 2 * c;
+                pv_of_token<B>(o[h][i], vf, hi[h], lo[h], r / group == tok, (r + 1) / group == tok);
+              }
+            }
+          }
+        }
+      }
+    }
+    // the key halves' results, eight rows at a time: the second half's warp gives, the first's joins and writes
+    const bool whole = t0 == 0 && t1 == now.nt;
+    float* part = parts + (t0 == 0 ? part_floats<R, DP>() : 0);
+    float* mine = give + wr * (Shape::kGive / 4) + lane;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float sum = l[h] + __shfl_xor_sync(~0u, l[h], 1);
+      sum += __shfl_xor_sync(~0u, sum, 2);
+      if (kh == 1) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mine[(i * 4 + j) * 32] = o[h][i][j];
+        mine[KS * 4 * 32] = m[h];
+        mine[(KS * 4 + 1) * 32] = sum;
+      }
+      __syncthreads();
+      if (kh == 0) {
+        const float m1 = mine[KS * 4 * 32], l1 = mine[(KS * 4 + 1) * 32];
+        const float top = fmaxf(m[h], m1), ref = top == ninf() ? 0.f : top;
+        const float g0 = ex2(m[h] - ref), g1 = ex2(m1 - ref);
+        const float total = g0 * sum + g1 * l1;
+        const int r0 = wrow0 + h * 8;
+        // the lane's columns are rows 2c and 2c + 1; what belongs to row n is with lane n * 4
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int from = c * 8 + j * 4, r = r0 + 2 * c + j;
+          const float f0 = __shfl_sync(~0u, g0, from), f1 = __shfl_sync(~0u, g1, from);
+          const float lr = __shfl_sync(~0u, total, from), tr = __shfl_sync(~0u, top, from);
+          const float inv = lr > 0.f ? 1.f / lr : (lr == 0.f ? 0.f : lr);
+          if (r >= a.rows) continue;
+          const RowAt at = row_at(a, seq, kvh, r);
+          T* out = static_cast<T*>(a.out) + at.out * a.head_dim;
+          float* pr = part + (r - row0) * DP;
+#pragma unroll
+          for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int d = i * 16 + x * 8 + n;
+              const float y = f0 * o[h][i][2 * x + j] + f1 * mine[(i * 4 + 2 * x + j) * 32];
+              if (!whole)
+                pr[d] = y;
+              else if (d < a.head_dim)
+                out[d] = from_f32<T>(y * inv);
+            }
+          if (n == 0) {
+            if (!whole)
+              *reinterpret_cast<float2*>(part + R * DP + 2 * (r - row0)) = make_float2(tr, lr);
+            else if (a.lse)
+              a.lse[at.out] = lr == 0.f ? ninf() : (tr + log2f(lr)) * 0.6931471805599453f;
+          }
+        }
+      }
+      __syncthreads();
     }
     cur += t1 - t0;
   }
@@ -724,7 +975,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_fma_kernel(const __grid_c
   const int units = a.n_kv_heads * row_tiles;
   const int range = blockIdx.x / units, unit = blockIdx.x - range * units;
   const int rt = unit / a.n_kv_heads, kvh = unit - rt * a.n_kv_heads, row0 = rt * R;
-  const Place pl = locate(a, range);
+  const Place pl = locate<kWarps>(a, range);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t chunk = chunk_of(pl.total, a.n_ranges);
   int64_t cur = int64_t(range) * chunk;
@@ -846,39 +1097,60 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __g
 struct Variant {
   const void* main;
   const void* join;
-  int rows;
+  int rows, threads;
   size_t smem, part;
 };
 
 template <typename T, int R, int DP>
 Variant tc() {
   return {reinterpret_cast<const void*>(&paged_attn_tc_kernel<T, R, DP>),
-          reinterpret_cast<const void*>(&paged_attn_join_kernel<T, R, DP>), R, TcShape<R, DP>::kSmem,
+          reinterpret_cast<const void*>(&paged_attn_join_kernel<T, R, DP>), R, kThreads, TcShape<R, DP>::kSmem,
           size_t(part_floats<R, DP>()) * sizeof(float)};
+}
+
+template <typename T, int WR, int DP>
+Variant shared_rows() {
+  return {reinterpret_cast<const void*>(&paged_attn_rows_kernel<T, WR, DP>),
+          reinterpret_cast<const void*>(&paged_attn_join_kernel<T, WR * 16, DP>), WR * 16, WR * 64,
+          RowsShape<WR, DP>::kSmem, size_t(part_floats<WR * 16, DP>()) * sizeof(float)};
 }
 
 template <typename T, int V, int DP>
 Variant fma_rows() {
   using Core = Fma<T, V, DP>;
   return {reinterpret_cast<const void*>(&paged_attn_fma_kernel<T, Core>),
-          reinterpret_cast<const void*>(&paged_attn_join_kernel<T, Core::kRows, DP>), Core::kRows,
+          reinterpret_cast<const void*>(&paged_attn_join_kernel<T, Core::kRows, DP>), Core::kRows, kThreads,
           sizeof(Merge<Core::kRows, DP>), size_t(part_floats<Core::kRows, DP>()) * sizeof(float)};
 }
 
-// [bf16, f16] x [8, 16, 40 query rows] x [64, 128, 256 elements] (40 rows of 256 do not
-// fit the registers), then f32 and the 16-bit types of any alignment.
-constexpr int kVariants = 24;
+// [bf16, f16] x ([8, 16 query rows] x [64, 128, 256 elements], [32, 48 rows] x [64, 128
+// elements]), then f32 and the 16-bit types of any alignment.
+constexpr int kVariants = 28;
+template <typename T>
+struct TcVariants {
+  static void fill(Variant* v) {
+    v[0] = tc<T, 8, 64>(), v[1] = tc<T, 8, 128>(), v[2] = tc<T, 8, 256>();
+    v[3] = tc<T, 16, 64>(), v[4] = tc<T, 16, 128>(), v[5] = tc<T, 16, 256>();
+    v[6] = shared_rows<T, 2, 64>(), v[7] = shared_rows<T, 2, 128>();
+    v[8] = shared_rows<T, 3, 64>(), v[9] = shared_rows<T, 3, 128>();
+  }
+};
+struct Variants {
+  Variant v[kVariants];
+  Variants() {
+    using bf = __nv_bfloat16;
+    using hf = __half;
+    TcVariants<bf>::fill(v);
+    TcVariants<hf>::fill(v + 10);
+    v[20] = fma_rows<float, 4, 128>(), v[21] = fma_rows<float, 4, 256>();
+    v[22] = fma_rows<float, 1, 128>(), v[23] = fma_rows<float, 1, 256>();
+    v[24] = fma_rows<bf, 1, 128>(), v[25] = fma_rows<bf, 1, 256>();
+    v[26] = fma_rows<hf, 1, 128>(), v[27] = fma_rows<hf, 1, 256>();
+  }
+};
 const Variant& variant_at(int i) {
-  using bf = __nv_bfloat16;
-  using hf = __half;
-  static const Variant v[kVariants] = {
-      tc<bf, 8, 64>(),  tc<bf, 8, 128>(),  tc<bf, 8, 256>(),  tc<bf, 16, 64>(), tc<bf, 16, 128>(), tc<bf, 16, 256>(),
-      tc<bf, 40, 64>(), tc<bf, 40, 128>(), tc<hf, 8, 64>(),   tc<hf, 8, 128>(), tc<hf, 8, 256>(),  tc<hf, 16, 64>(),
-      tc<hf, 16, 128>(), tc<hf, 16, 256>(), tc<hf, 40, 64>(), tc<hf, 40, 128>(),
-      fma_rows<float, 4, 128>(), fma_rows<float, 4, 256>(), fma_rows<float, 1, 128>(), fma_rows<float, 1, 256>(),
-      fma_rows<bf, 1, 128>(),    fma_rows<bf, 1, 256>(),    fma_rows<hf, 1, 128>(),    fma_rows<hf, 1, 256>(),
-  };
-  return v[i];
+  static const Variants all;
+  return all.v[i];
 }
 
 }  // namespace
@@ -893,7 +1165,7 @@ cudaError_t plan_variant(int v, int n_kv_heads, int rows, int n_sm, AttnPlan* pl
     cudaError_t e = cudaSuccess;
     if (k.smem > 48 * 1024)
       e = cudaFuncSetAttribute(k.main, cudaFuncAttributeMaxDynamicSharedMemorySize, int(k.smem));
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k.main, kThreads, k.smem);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k.main, k.threads, k.smem);
     if (e != cudaSuccess) return e;
     if (n < 1) return cudaErrorInvalidConfiguration;
     __atomic_store_n(&resident[v], n, __ATOMIC_RELAXED);
@@ -916,10 +1188,13 @@ cudaError_t plan_variant(int v, int n_kv_heads, int rows, int n_sm, AttnPlan* pl
 int variant_for(const AttnArgs& a, int dtype, bool wide) {
   if (dtype != 1 && wide) {
     const int size = a.head_dim <= 64 ? 0 : a.head_dim <= 128 ? 1 : 2;
-    const int tile = a.rows <= 8 ? 0 : a.rows <= 16 || size == 2 ? 1 : 2;
-    return (dtype == 0 ? 0 : 8) + tile * 3 + size;
+    const int first = dtype == 0 ? 0 : 10;
+    if (a.rows <= 8) return first + size;
+    if (a.rows <= 16 || size == 2) return first + 3 + size;
+    // 32 or 48 rows a unit: whichever reads the keys in fewer units, then the smaller
+    return first + ((a.rows + 31) / 32 <= (a.rows + 47) / 48 ? 6 : 8) + size;
   }
-  return (dtype == 1 ? (wide ? 16 : 18) : dtype == 0 ? 20 : 22) + (a.head_dim <= 128 ? 0 : 1);
+  return (dtype == 1 ? (wide ? 20 : 22) : dtype == 0 ? 24 : 26) + (a.head_dim <= 128 ? 0 : 1);
 }
 
 }  // namespace
@@ -952,7 +1227,7 @@ cudaError_t launch_paged_attn(const AttnArgs& args, const AttnPlan& plan, cudaSt
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(plan.n_workers));
   a.n_ranges = plan.n_ranges;
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(unsigned(k.threads));
   cfg.dynamicSmemBytes = k.smem;
   cfg.stream = s;
   cudaError_t e = cudaLaunchKernelExC(&cfg, k.main, params);
