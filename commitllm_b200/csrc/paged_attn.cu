@@ -7,8 +7,9 @@
 // read once, for 4 * n_new * group operations per element (group = query heads
 // of one KV head), far under the tensor cores' rate for a few new tokens.
 //
-// Work split.  All sequences' keys, in tiles of 64, are laid end to end and cut
-// into equal contiguous ranges; a worker CTA takes one range for one unit (KV
+// Work split.  All sequences' keys, in tiles of 64 (and what starting a sequence costs,
+// counted as tiles), are laid end to end and cut into equal contiguous ranges; a worker
+// CTA takes one range for one unit (KV
 // head, tile of up to R query rows).  The number of ranges is set so that the
 // workers are all resident at once, so a ragged batch and a single long sequence
 // both spread evenly without the host knowing the lengths.  The units of a range
@@ -44,8 +45,17 @@ __device__ __forceinline__ int64_t seq_len(const AttnArgs& a, int s) {
   return n < 0 ? 0 : (n > cap ? cap : n);
 }
 
-__device__ __forceinline__ int64_t seq_tiles(const AttnArgs& a, int s) {
+__device__ __forceinline__ int64_t key_tiles(const AttnArgs& a, int s) {
   return (seq_len(a, s) + kTile - 1) / kTile;
+}
+
+// What a sequence counts for when the ranges are cut: kStart tiles for starting it
+// (queries to read, a result to write: about two tiles' time) and its keys' tiles
+// behind them.
+constexpr int kStart = 2;
+__device__ __forceinline__ int64_t seq_tiles(const AttnArgs& a, int s) {
+  const int64_t n = key_tiles(a, s);
+  return n ? n + kStart : 0;
 }
 
 // Inclusive sum of v over the block's W warps.
@@ -120,6 +130,24 @@ __device__ Place locate(const AttnArgs& a, int range) {
   return pl;
 }
 
+// The sequence that holds a tile, and what a warp needs of it.
+struct Cursor {
+  int seq, len, nt;
+  int64_t base;       // its first tile of keys
+  __device__ __forceinline__ void at(const AttnArgs& a, int s, int64_t b) {
+    seq = s, base = b;
+    len = int(seq_len(a, s));
+    nt = (len + kTile - 1) / kTile;
+    if (nt) base += kStart;
+  }
+  // The first tile of keys from `tile` on, if it is before `end`; else end.
+  __device__ __forceinline__ int64_t advance(const AttnArgs& a, int64_t tile, int64_t end) {
+    while (tile < end && tile >= base + nt) at(a, seq + 1, base + nt);
+    if (tile < base) tile = base;
+    return tile < end ? tile : end;
+  }
+};
+
 // Element offset of the row of key p, or -1 (a bad page, reported through err).
 __device__ __forceinline__ int64_t row_of(const AttnArgs& a, int seq, int p) {
   const int block = unsigned(p) / unsigned(a.block_size);
@@ -156,16 +184,6 @@ __device__ __forceinline__ RowAt row_at(const AttnArgs& a, int seq, int kvh, int
 // A part in the workspace: R rows of DP outputs, then R x (maximum, sum).
 template <int R, int DP> constexpr int64_t part_floats() { return int64_t(R) * DP + 2 * R; }
 
-// Shared memory of a unit's end: each warp's outputs, maxima (base-2 exponents) and
-// sums, R rows at a time.  Rows are padded by 16 bytes: a warp's stores then fall
-// into different banks.
-template <int R, int DP>
-struct Merge {
-  float o[kWarps][R][DP + 4];
-  float m[kWarps][R];
-  float l[kWarps][R];
-};
-
 // 2^x for x <= 0, within 2^-22 of itself; nothing below 2^-126.
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -173,45 +191,95 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// The warps' results of R rows from row0, joined and written: the outputs, or a part
-// (whose rows are at `rows` and whose maxima and sums at `ml`).
-template <typename T, int R, int DP>
-__device__ __forceinline__ void emit(const AttnArgs& a, Merge<R, DP>& mg, int seq, int kvh, int row0, bool whole,
-                                     float* rows, float* ml) {
+// Shared memory of a unit's end: the outputs of R rows from W warps that saw different
+// keys, D elements at a time, with their maxima (base-2 exponents) and sums.  Rows are
+// padded by 16 bytes: a warp's stores then fall into different banks.
+template <int W, int R, int D>
+struct Merge {
+  float o[W][R][D + 4];
+  float m[W][R];       // then the factors of the warps' outputs
+  float l[W][R];
+  int64_t at[R];       // where the row goes (elements of out or of the part), -1: nowhere
+};
+
+// Where a unit's rows go: the outputs, or (part not null) a part of DP-element rows
+// whose maxima and sums follow at ml.
+struct Target {
+  int seq, kvh, row0;
+  float* part;
+  float* ml;
+};
+
+// The W warps' results, joined and written, elements d0.. of each row; `first`: the
+// maxima and sums are new.  Buffer row b is query row row0 + (b / 8) * step + b % 8.
+// One copy of the code for all its uses: it runs once a unit, and code that runs once
+// costs its fetching (inlined and unrolled it made a short call microseconds longer).
+template <typename T, int W, int R, int D, int DP>
+__device__ __noinline__ void emit(const AttnArgs& a, Merge<W, R, D>& mg, Target to, int step, bool first, int d0) {
   __syncthreads();
-  constexpr int kPer = R * DP / 4;     // float4 groups
-  for (int i = threadIdx.x; i < kPer; i += kThreads) {
-    const int r = i / (DP / 4), d = (i - r * (DP / 4)) * 4;
-    float top = mg.m[0][r];
+  if (first) {
+    const int b = threadIdx.x;
+    if (b < R) {
+      const int r = (b >> 3) * step + (b & 7);
+      float top = mg.m[0][b];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, mg.m[w][r]);
-    const float ref = top == ninf() ? 0.f : top;
+      for (int w = 1; w < W; ++w) top = fmaxf(top, mg.m[w][b]);
+      const float ref = top == ninf() ? 0.f : top;
+      float f[W], l = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        f[w] = ex2(mg.m[w][b] - ref);
+        l += f[w] * mg.l[w][b];
+      }
+      float inv = 1.f;
+      int64_t at = -1;
+      if (to.part) {
+        *reinterpret_cast<float2*>(to.ml + 2 * r) = make_float2(top, l);
+        at = int64_t(r) * DP;
+      } else {
+        inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);     // a NaN sum stays NaN
+        if (to.row0 + r < a.rows) {
+          const RowAt ra = row_at(a, to.seq, to.kvh, to.row0 + r);
+          at = ra.out * a.head_dim;
+          if (a.lse) a.lse[ra.out] = l == 0.f ? ninf() : (top + log2f(l)) * 0.6931471805599453f;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < W; ++w) mg.m[w][b] = f[w] * inv;
+      mg.at[b] = at;
+    }
+    __syncthreads();
+  }
+#pragma unroll 2
+  for (int i = threadIdx.x; i < R * D / 4; i += blockDim.x) {
+    const int b = i / (D / 4), e = (i - b * (D / 4)) * 4, d = d0 + e;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = ex2(mg.m[w][r] - ref);
-      l += f * mg.l[w][r];
-      const float4 x = *reinterpret_cast<const float4*>(&mg.o[w][r][d]);
+    for (int w = 0; w < W; ++w) {
+      const float f = mg.m[w][b];
+      const float4 x = *reinterpret_cast<const float4*>(&mg.o[w][b][e]);
       o.x += f * x.x;
       o.y += f * x.y;
       o.z += f * x.z;
       o.w += f * x.w;
     }
-    if (!whole) {
-      *reinterpret_cast<float4*>(rows + r * DP + d) = o;
-      if (d == 0) *reinterpret_cast<float2*>(ml + 2 * r) = make_float2(top, l);
-      continue;
-    }
-    if (row0 + r >= a.rows || d >= a.head_dim) continue;
-    const RowAt at = row_at(a, seq, kvh, row0 + r);
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);     // a NaN sum stays NaN
-    T* out = static_cast<T*>(a.out) + at.out * a.head_dim + d;
-    const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    const int64_t at = mg.at[b];
+    if (to.part) {
+      *reinterpret_cast<float4*>(to.part + at + d) = o;
+    } else if (at >= 0 && d < a.head_dim) {
+      T* out = static_cast<T*>(a.out) + at + d;
+      const float y[4] = {o.x, o.y, o.z, o.w};
+      if (d + 4 <= a.head_dim && a.wide_out) {
+        struct alignas(4 * sizeof(T)) Four {
+          T v[4];
+        } four = {{from_f32<T>(y[0]), from_f32<T>(y[1]), from_f32<T>(y[2]), from_f32<T>(y[3])}};
+        *reinterpret_cast<Four*>(out) = four;
+      } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (d + e < a.head_dim) out[e] = from_f32<T>(y[e]);
-    if (d == 0 && a.lse) a.lse[at.out] = l == 0.f ? ninf() : (top + log2f(l)) * 0.6931471805599453f;
+        for (int j = 0; j < 4; ++j)
+          if (d + j < a.head_dim) out[j] = from_f32<T>(y[j]);
+      }
+    }
   }
   __syncthreads();
 }
@@ -267,20 +335,6 @@ __device__ __forceinline__ void ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 
-// The sequence that holds a tile, and what a warp needs of it.
-struct Cursor {
-  int seq, len, nt;
-  int64_t base;       // its first tile
-  __device__ __forceinline__ void at(const AttnArgs& a, int s, int64_t b) {
-    seq = s, base = b;
-    len = int(seq_len(a, s));
-    nt = (len + kTile - 1) / kTile;
-  }
-  __device__ __forceinline__ void advance(const AttnArgs& a, int64_t tile) {
-    while (tile >= base + nt) at(a, seq + 1, base + nt);
-  }
-};
-
 // What one worker keeps in shared memory: a ring of stages a warp (16 keys' K rows,
 // then their V rows), then what the end of a unit needs.
 template <int R, int DP>
@@ -288,12 +342,12 @@ struct TcShape {
   static constexpr int kStage = 16 * DP * 2 * 2;
   static constexpr int kStages = DP == 64 ? 6 : 3;      // 96 KB a CTA (DP = 256: 192 KB)
   static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr size_t kSmem = kRing + sizeof(Merge<8, DP>);
+  static constexpr size_t kSmem = kRing + sizeof(Merge<kWarps, 8, DP>);
 };
 
 // Whether n 16-byte chunks of shared memory hold an infinity or a NaN (by the whole warp).
 template <typename B>
-__device__ __forceinline__ bool not_finite(uint32_t addr, int n) {
+__device__ __noinline__ bool not_finite(uint32_t addr, int n) {
   bool bad = false;
 #pragma unroll 1
   for (int i = threadIdx.x & 31; i < n; i += 32) {
@@ -327,25 +381,32 @@ __device__ __forceinline__ void pv_of_token(float (&o)[4], const uint32_t (&vf)[
 // no weight passes 2^8, which f16 holds too.
 constexpr float kSlack = 8.f;
 
-// Scores to weights for one column tile of 8 query rows (the lane's: lane / 4) and 16 keys
-// (the lane's: 2c, 2c + 1, 2c + 8, 2c + 9; those from `left` after 2c on are not seen):
-// the running reference and sum, the sums so far where the reference moves, and the
-// weights in two 16-bit parts.
-template <typename B, int KS>
-__device__ __forceinline__ void weigh(const float (&s)[2][2], float scale, int left, int c, float& m, float& l,
-                                      float (&o)[KS][4], uint32_t (&hi)[2], uint32_t (&lo)[2]) {
-  float x[2][2], top = ninf();
+// Scores to weights for one column tile of 8 query rows (the lane's: lane / 4) and NB
+// blocks of 16 keys (the lane's of block b: 16b + 2c + {0, 1, 8, 9}; those from `left`
+// after 2c on are not seen): the running reference and sum, the sums so far where the
+// reference moves, and the weights in two 16-bit parts.  A lane compares only its own
+// scores with the reference; the row's maximum is exchanged where one of them passes
+// it.  scale is not negative.
+template <typename B, int NB, int KS>
+__device__ __forceinline__ void weigh(float (&s)[NB][2][2], float scale, bool all_seen, int left, int c, float& m, float& l,
+                                      float (&o)[KS][4], uint32_t (&hi)[NB][2], uint32_t (&lo)[NB][2]) {
+  if (!all_seen) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      x[i][j] = 8 * i + j < left ? s[i][j] * scale : ninf();
-      top = fmaxf(top, x[i][j]);
-    }
-  top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-  top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (16 * b + 8 * i + j >= left) s[b][i][j] = ninf();
+  }
+  float top = ninf();
+#pragma unroll
+  for (int b = 0; b < NB; ++b) top = fmaxf(top, fmaxf(fmaxf(s[b][0][0], s[b][0][1]), fmaxf(s[b][1][0], s[b][1][1])));
+  top = top == ninf() ? top : top * scale;       // (-infinity * 0)
   if (__any_sync(~0u, top > m + kSlack)) {
     // what is summed so far shrinks to the new maximum
+    top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
     top = fmaxf(top, m);
     const float f = m == ninf() ? 0.f : ex2(m - top);
     l *= f;
@@ -359,13 +420,20 @@ __device__ __forceinline__ void weigh(const float (&s)[2][2], float scale, int l
   }
   const float ref = m == ninf() ? 0.f : m;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float e0 = ex2(x[i][0] - ref), e1 = ex2(x[i][1] - ref);
-    l += e0 + e1;
-    hi[i] = B::pack(e0, e1);
-    const float2 h = B::unpack(hi[i]);
-    lo[i] = B::pack(e0 - h.x, e1 - h.y);
-  }
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float e[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        e[j] = ex2(fmaf(s[b][i][j], scale, -ref));
+        if (!all_seen && 16 * b + 8 * i + j >= left) e[j] = 0.f;
+      }
+      l += e[0] + e[1];
+      hi[b][i] = B::pack(e[0], e[1]);
+      const float2 h = B::unpack(hi[b][i]);
+      lo[b][i] = B::pack(e[0] - h.x, e[1] - h.y);
+    }
 }
 
 // Attention of up to R query rows on the tensor cores, K and V rows of 16-bit types.
@@ -395,7 +463,8 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
   constexpr int kCols = DP / 8;        // 16-byte chunks of a row
   constexpr int kRowsPerCopy = 32 / kCols > 0 ? 32 / kCols : 1;
   extern __shared__ __align__(128) char smem[];
-  Merge<8, DP>& mg = *reinterpret_cast<Merge<8, DP>*>(smem + Shape::kRing);
+  using Mg = Merge<kWarps, 8, DP>;
+  Mg& mg = *reinterpret_cast<Mg*>(smem + Shape::kRing);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
   const uint32_t ring = smem_addr(smem) + warp * (kStages * Shape::kStage);
   const int row_tiles = (a.rows + R - 1) / R;
@@ -419,8 +488,8 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
   bool real = false;
   auto look = [&]() {
     real = false;
+    next = ahead.advance(a, next, end);
     if (next < end) {
-      ahead.advance(a, next);
       const int p = int(next - ahead.base) * kTile + warp * 16 + lane;
       if (lane < 16 && p < ahead.len) {
         const int block = unsigned(p) / unsigned(a.block_size);
@@ -474,8 +543,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
   Cursor now;
   now.at(a, pl.seq, pl.seq_base);
   int64_t cur = begin;
-  while (cur < end) {
-    now.advance(a, cur);
+  while ((cur = now.advance(a, cur, end)) < end) {
     const int seq = now.seq, len = now.len;
     const int t0 = int(cur - now.base);
     const int t1 = now.nt - t0 < end - cur ? now.nt : t0 + int(end - cur);
@@ -489,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const int e = ks * 16 + x * 8 + 2 * c;
-            q[ks][h + 2 * x] = has && e < a.head_dim ? *reinterpret_cast<const uint32_t*>(src + e) : 0u;
+            q[ks][h + 2 * x] = has && e < a.head_dim ? *reinterpret_cast<const uint32_t*>(src + e) ^ a.q_sign : 0u;
           }
       }
 #pragma unroll
@@ -523,11 +591,11 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
       }
       const int sure = len - a.n_new + 1;        // every row sees the keys before it
       const bool all_seen = p0 + 16 <= sure;
-      uint32_t hi[NT][2], lo[NT][2];
+      uint32_t hi[NT][1][2], lo[NT][1][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const float x[2][2] = {{s[0][t * 2], s[0][t * 2 + 1]}, {s[1][t * 2], s[1][t * 2 + 1]}};
-        weigh<B, KS>(x, a.scale_log2, all_seen ? 0x7fffffff : lim[t] - p0 - 2 * c, c, m[t], l[t], o[t], hi[t], lo[t]);
+        float x[1][2][2] = {{{s[0][t * 2], s[0][t * 2 + 1]}, {s[1][t * 2], s[1][t * 2 + 1]}}};
+        weigh<B, 1, KS>(x, a.scale_log2, all_seen, lim[t] - p0 - 2 * c, c, m[t], l[t], o[t], hi[t], lo[t]);
       }
       const uint32_t vrow = vst + key * (DP * 2);
       // Rows that see different keys share this tile: 0 * infinity of a value that only
@@ -541,9 +609,9 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
           if (i + 1 < KS) ldsm_t(vrow + ((((i + 1) * 2 + half) ^ flip) << 4), vf[(i + 1) & 1]);
           const uint32_t(&v)[4] = vf[i & 1];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) B::mma(o[t][i], v[0], v[1], v[2], v[3], hi[t][0], hi[t][1]);
+          for (int t = 0; t < NT; ++t) B::mma(o[t][i], v[0], v[1], v[2], v[3], hi[t][0][0], hi[t][0][1]);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) B::mma(o[t][i], v[0], v[1], v[2], v[3], lo[t][0], lo[t][1]);
+          for (int t = 0; t < NT; ++t) B::mma(o[t][i], v[0], v[1], v[2], v[3], lo[t][0][0], lo[t][0][1]);
         }
       } else {
         // token by token: keys that it does not see become zeros, and only its columns are kept
@@ -558,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               const int r = row0 + t * 8 + 2 * c;
-              pv_of_token<B>(o[t][i], vf, hi[t], lo[t], r / group == tok, (r + 1) / group == tok);
+              pv_of_token<B>(o[t][i], vf, hi[t][0], lo[t][0], r / group == tok, (r + 1) / group == tok);
             }
           }
         }
@@ -577,7 +645,8 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
       for (int i = 0; i < KS; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) mg.o[warp][2 * c + (j & 1)][i * 16 + (j >> 1) * 8 + n] = o[t][i][j];
-      emit<T, 8, DP>(a, mg, seq, kvh, row0 + t * 8, whole, part + t * 8 * DP, part + R * DP + t * 16);
+      emit<T, kWarps, 8, DP, DP>(a, mg, {seq, kvh, row0 + t * 8, whole ? nullptr : part + t * 8 * DP, part + R * DP + t * 16}, 8,
+                                 true, 0);
     }
     cur += t1 - t0;
   }
@@ -595,9 +664,8 @@ struct RowsShape {
   static constexpr int kStage = kTile * DP * 2 * 2;
   static constexpr int kStages = DP == 64 ? 6 : 3;
   static constexpr int kRing = kStages * kStage;             // 96 KB
-  // a key half's results of 8 rows, as its lanes hold them: outputs, maximum, sum
-  static constexpr int kGive = (DP / 16 * 4 + 2) * 32 * 4;
-  static constexpr size_t kSmem = kRing + WR * kGive;
+  using Mg = Merge<2, WR * 8, DP / 2>;      // 8 rows of each row tile, half of their elements
+  static constexpr size_t kSmem = kRing + sizeof(Mg);
 };
 
 template <typename T, int WR, int DP>
@@ -611,7 +679,7 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
   constexpr int kRowsPerCopy = 32 / kCols;
   constexpr int kCopies = (kTile / kRowsPerCopy + kW - 1) / kW;      // a warp's, of K and of V
   extern __shared__ __align__(128) char smem[];
-  float* give = reinterpret_cast<float*>(smem + Shape::kRing);
+  typename Shape::Mg& mg = *reinterpret_cast<typename Shape::Mg*>(smem + Shape::kRing);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
   const int wr = warp >> 1, kh = warp & 1;
   const uint32_t ring = smem_addr(smem);
@@ -638,8 +706,8 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
   const int my_group = warp + lane / kRowsPerCopy * kW, my_row = my_group * kRowsPerCopy + lane % kRowsPerCopy;
   auto look = [&]() {
     real = false;
+    next = ahead.advance(a, next, end);
     if (next < end) {
-      ahead.advance(a, next);
       const int p = int(next - ahead.base) * kTile + my_row;
       if (lane < kCopies * kRowsPerCopy && my_row < kTile && p < ahead.len) {
         const int block = unsigned(p) / unsigned(a.block_size);
@@ -693,8 +761,7 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
   Cursor now;
   now.at(a, pl.seq, pl.seq_base);
   int64_t cur = begin;
-  while (cur < end) {
-    now.advance(a, cur);
+  while ((cur = now.advance(a, cur, end)) < end) {
     const int seq = now.seq, len = now.len;
     const int t0 = int(cur - now.base);
     const int t1 = now.nt - t0 < end - cur ? now.nt : t0 + int(end - cur);
@@ -708,7 +775,7 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int e = ks * 16 + x * 8 + 2 * c;
-          q[ks][h + 2 * x] = has && e < a.head_dim ? *reinterpret_cast<const uint32_t*>(src + e) : 0u;
+          q[ks][h + 2 * x] = has && e < a.head_dim ? *reinterpret_cast<const uint32_t*>(src + e) ^ a.q_sign : 0u;
         }
       lim[h] = has ? len - a.n_new + 1 + r / group : 0;
       m[h] = ninf();
@@ -726,115 +793,87 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
       const uint32_t kst = ring + use * Shape::kStage, vst = kst + kTile * DP * 2;
       use = use + 1 == kStages ? 0 : use + 1;
       const int sure = len - a.n_new + 1;
-#pragma unroll 1
-      for (int b = 0; b < 2; ++b) {
-        const int at = kh * 32 + b * 16;               // rows of the stage
-        const int p0 = t * kTile + at;
-        const uint32_t krow = kst + (at + key) * (DP * 2), vrow = vst + (at + key) * (DP * 2);
-        float s[2][4] = {};
-        uint32_t kf[2][4];
-        ldsm(krow + ((half ^ flip) << 4), kf[0]);
+      // the warp's 32 keys as two blocks of 16 side by side: four independent chains of products
+      const int at = kh * 32, p0 = t * kTile + at;     // rows of the stage
+      const uint32_t krow = kst + (at + key) * (DP * 2), vrow = vst + (at + key) * (DP * 2);
+      constexpr uint32_t kBlock = 16 * DP * 2;
+      float s[2][2][4] = {};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          if (ks + 1 < KS) ldsm(krow + ((((ks + 1) * 2 + half) ^ flip) << 4), kf[(ks + 1) & 1]);
-          const uint32_t(&k)[4] = kf[ks & 1];
-          B::mma(s[0], q[ks][0], q[ks][1], q[ks][2], q[ks][3], k[0], k[1]);
-          B::mma(s[1], q[ks][0], q[ks][1], q[ks][2], q[ks][3], k[2], k[3]);
-        }
-        const bool all_seen = p0 + 16 <= sure;
-        uint32_t hi[2][2], lo[2][2];
+      for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float x[2][2] = {{s[0][h * 2], s[0][h * 2 + 1]}, {s[1][h * 2], s[1][h * 2 + 1]}};
-          weigh<B, KS>(x, a.scale_log2, all_seen ? 0x7fffffff : lim[h] - p0 - 2 * c, c, m[h], l[h], o[h], hi[h], lo[h]);
+        for (int b = 0; b < 2; ++b) {
+          uint32_t k[4];
+          ldsm(krow + b * kBlock + (((ks * 2 + half) ^ flip) << 4), k);
+          B::mma(s[b][0], q[ks][0], q[ks][1], q[ks][2], q[ks][3], k[0], k[1]);
+          B::mma(s[b][1], q[ks][0], q[ks][1], q[ks][2], q[ks][3], k[2], k[3]);
         }
-        // rows that see different keys share this tile: see paged_attn_tc_kernel
-        const bool wild = !all_seen && a.n_new > 1 && not_finite<B>(vst + at * (DP * 2), 16 * kCols);
-        if (!wild) {
-          uint32_t vf[2][4];
-          ldsm_t(vrow + ((half ^ flip) << 4), vf[0]);
+      }
+      const bool all_seen = p0 + 32 <= sure;
+      uint32_t hi[2][2][2], lo[2][2][2];               // [column tile][block]
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float x[2][2][2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) x[b][i][0] = s[b][i][h * 2], x[b][i][1] = s[b][i][h * 2 + 1];
+        weigh<B, 2, KS>(x, a.scale_log2, all_seen, lim[h] - p0 - 2 * c, c, m[h], l[h], o[h], hi[h], lo[h]);
+      }
+      // rows that see different keys share this tile: see paged_attn_tc_kernel
+      const bool wild = !all_seen && a.n_new > 1 && not_finite<B>(vst + at * (DP * 2), 32 * kCols);
+      if (!wild) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int i = 0; i < KS; ++i) {
-            if (i + 1 < KS) ldsm_t(vrow + ((((i + 1) * 2 + half) ^ flip) << 4), vf[(i + 1) & 1]);
-            const uint32_t(&v)[4] = vf[i & 1];
+            uint32_t v[4];
+            ldsm_t(vrow + b * kBlock + (((i * 2 + half) ^ flip) << 4), v);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) B::mma(o[h][i], v[0], v[1], v[2], v[3], hi[h][0], hi[h][1]);
+            for (int h = 0; h < 2; ++h) B::mma(o[h][i], v[0], v[1], v[2], v[3], hi[h][b][0], hi[h][b][1]);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) B::mma(o[h][i], v[0], v[1], v[2], v[3], lo[h][0], lo[h][1]);
+            for (int h = 0; h < 2; ++h) B::mma(o[h][i], v[0], v[1], v[2], v[3], lo[h][b][0], lo[h][b][1]);
           }
-        } else {
+      } else {
 #pragma unroll 1
-          for (int tok = wrow0 / group; tok < a.n_new && tok * group < wrow0 + 16; ++tok) {
-            const uint32_t m0 = seen_pair(p0 + 2 * c, sure + tok), m1 = seen_pair(p0 + 2 * c + 8, sure + tok);
+        for (int tok = wrow0 / group; tok < a.n_new && tok * group < wrow0 + 16; ++tok) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const int pb = p0 + 16 * b + 2 * c;
+            const uint32_t m0 = seen_pair(pb, sure + tok), m1 = seen_pair(pb + 8, sure + tok);
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
               uint32_t vf[4];
-              ldsm_t(vrow + (((i * 2 + half) ^ flip) << 4), vf);
+              ldsm_t(vrow + b * kBlock + (((i * 2 + half) ^ flip) << 4), vf);
               vf[0] &= m0, vf[1] &= m0, vf[2] &= m1, vf[3] &= m1;
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const int r = wrow0 + h * 8 + 2 * c;
-                pv_of_token<B>(o[h][i], vf, hi[h], lo[h], r / group == tok, (r + 1) / group == tok);
+                pv_of_token<B>(o[h][i], vf, hi[h][b], lo[h][b], r / group == tok, (r + 1) / group == tok);
               }
             }
           }
         }
       }
     }
-    // the key halves' results, eight rows at a time: the second half's warp gives, the first's joins and writes
+    // the key halves' results: query rows 0-7 or 8-15 of each row tile, and half of their
+    // elements, at a time; buffer row 8 * wr + n is query row row0 + 16 * wr + 8 * h + n
     const bool whole = t0 == 0 && t1 == now.nt;
     float* part = parts + (t0 == 0 ? part_floats<R, DP>() : 0);
-    float* mine = give + wr * (Shape::kGive / 4) + lane;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float sum = l[h] + __shfl_xor_sync(~0u, l[h], 1);
       sum += __shfl_xor_sync(~0u, sum, 2);
-      if (kh == 1) {
+      if (c == 0) mg.m[kh][wr * 8 + n] = m[h], mg.l[kh][wr * 8 + n] = sum;
 #pragma unroll
-        for (int i = 0; i < KS; ++i)
+      for (int z = 0; z < 2; ++z) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mine[(i * 4 + j) * 32] = o[h][i][j];
-        mine[KS * 4 * 32] = m[h];
-        mine[(KS * 4 + 1) * 32] = sum;
+        for (int i = 0; i < KS / 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mg.o[kh][wr * 8 + 2 * c + (j & 1)][i * 16 + (j >> 1) * 8 + n] = o[h][z * (KS / 2) + i][j];
+        emit<T, 2, WR * 8, DP / 2, DP>(a, mg, {seq, kvh, row0 + 8 * h, whole ? nullptr : part + 8 * h * DP, part + R * DP + 16 * h}, 16,
+                                       z == 0, z * (DP / 2));
       }
-      __syncthreads();
-      if (kh == 0) {
-        const float m1 = mine[KS * 4 * 32], l1 = mine[(KS * 4 + 1) * 32];
-        const float top = fmaxf(m[h], m1), ref = top == ninf() ? 0.f : top;
-        const float g0 = ex2(m[h] - ref), g1 = ex2(m1 - ref);
-        const float total = g0 * sum + g1 * l1;
-        const int r0 = wrow0 + h * 8;
-        // the lane's columns are rows 2c and 2c + 1; what belongs to row n is with lane n * 4
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int from = c * 8 + j * 4, r = r0 + 2 * c + j;
-          const float f0 = __shfl_sync(~0u, g0, from), f1 = __shfl_sync(~0u, g1, from);
-          const float lr = __shfl_sync(~0u, total, from), tr = __shfl_sync(~0u, top, from);
-          const float inv = lr > 0.f ? 1.f / lr : (lr == 0.f ? 0.f : lr);
-          if (r >= a.rows) continue;
-          const RowAt at = row_at(a, seq, kvh, r);
-          T* out = static_cast<T*>(a.out) + at.out * a.head_dim;
-          float* pr = part + (r - row0) * DP;
-#pragma unroll
-          for (int i = 0; i < KS; ++i)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int d = i * 16 + x * 8 + n;
-              const float y = f0 * o[h][i][2 * x + j] + f1 * mine[(i * 4 + 2 * x + j) * 32];
-              if (!whole)
-                pr[d] = y;
-              else if (d < a.head_dim)
-                out[d] = from_f32<T>(y * inv);
-            }
-          if (n == 0) {
-            if (!whole)
-              *reinterpret_cast<float2*>(part + R * DP + 2 * (r - row0)) = make_float2(tr, lr);
-            else if (a.lse)
-              a.lse[at.out] = lr == 0.f ? ninf() : (tr + log2f(lr)) * 0.6931471805599453f;
-          }
-        }
-      }
-      __syncthreads();
     }
     cur += t1 - t0;
   }
@@ -939,7 +978,7 @@ struct Fma {
     }
   }
 
-  __device__ __forceinline__ void store(Merge<R, DP>& mg) {
+  __device__ __forceinline__ void store(Merge<kWarps, R, DP>& mg) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane & 7;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -970,7 +1009,8 @@ template <typename T, typename Core>
 __global__ void __launch_bounds__(kThreads) paged_attn_fma_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int R = Core::kRows, DP = Core::kDP;
   extern __shared__ __align__(128) char smem[];
-  Merge<R, DP>& mg = *reinterpret_cast<Merge<R, DP>*>(smem);
+  using Mg = Merge<kWarps, R, DP>;
+  Mg& mg = *reinterpret_cast<Mg*>(smem);
   const int row_tiles = (a.rows + R - 1) / R;
   const int units = a.n_kv_heads * row_tiles;
   const int range = blockIdx.x / units, unit = blockIdx.x - range * units;
@@ -980,26 +1020,21 @@ __global__ void __launch_bounds__(kThreads) paged_attn_fma_kernel(const __grid_c
   const int64_t chunk = chunk_of(pl.total, a.n_ranges);
   int64_t cur = int64_t(range) * chunk;
   const int64_t end = cur + chunk < pl.total ? cur + chunk : pl.total;
-  int seq = pl.seq;
-  int64_t base = pl.seq_base;
+  Cursor now;
+  now.at(a, pl.seq, pl.seq_base);
   float* parts = a.parts + int64_t(blockIdx.x) * 2 * part_floats<R, DP>();
-  while (cur < end) {
-    const int64_t nt = seq_tiles(a, seq);
-    if (cur >= base + nt) {
-      base += nt;
-      ++seq;
-      continue;
-    }
-    const int t0 = int(cur - base);
-    const int t1 = nt - t0 < end - cur ? int(nt) : t0 + int(end - cur);
-    const int len = int(seq_len(a, seq));
+  if (cur >= end) return;
+  while ((cur = now.advance(a, cur, end)) < end) {
+    const int seq = now.seq, len = now.len, nt = now.nt;
+    const int t0 = int(cur - now.base);
+    const int t1 = nt - t0 < end - cur ? nt : t0 + int(end - cur);
     Core core;
     core.run(a, seq, kvh, row0, len, t0, t1, mg.o[0]);      // the queries sit where the outputs will
     __syncthreads();
     core.store(mg);
     // a part that begins its sequence goes to slot 1, one that continues it to slot 0
     float* part = parts + (t0 == 0 ? part_floats<R, DP>() : 0);
-    emit<T, R, DP>(a, mg, seq, kvh, row0, t0 == 0 && t1 == nt, part, part + R * DP);
+    emit<T, kWarps, R, DP, DP>(a, mg, {seq, kvh, row0, t0 == 0 && t1 == nt ? nullptr : part, part + R * DP}, 8, true, 0);
     cur += t1 - t0;
   }
 }
@@ -1035,7 +1070,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __g
   if (lane == 0) warp_sum[warp] = before;
   __syncthreads();
   before = warp_sum[0] + warp_sum[1] + warp_sum[2] + warp_sum[3];
-  const int64_t nt = seq_tiles(a, seq);
+  const int64_t nt = key_tiles(a, seq);
   const RowAt at = row_at(a, seq, kvh, row);
   T* out = static_cast<T*>(a.out) + at.out * a.head_dim;
   if (nt == 0) {
@@ -1046,6 +1081,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __g
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (nt == 0) return;
   const int64_t chunk = chunk_of(total, a.n_ranges);
+  before += kStart;
   const int64_t wa = before / chunk, wb = (before + nt - 1) / chunk;
   if (wa == wb) return;
   const int r = row % R;
@@ -1098,20 +1134,23 @@ struct Variant {
   const void* main;
   const void* join;
   int rows, threads;
+  bool tensor;
+  size_t esz;
   size_t smem, part;
 };
 
 template <typename T, int R, int DP>
 Variant tc() {
   return {reinterpret_cast<const void*>(&paged_attn_tc_kernel<T, R, DP>),
-          reinterpret_cast<const void*>(&paged_attn_join_kernel<T, R, DP>), R, kThreads, TcShape<R, DP>::kSmem,
+          reinterpret_cast<const void*>(&paged_attn_join_kernel<T, R, DP>), R, kThreads, true, sizeof(T),
+          TcShape<R, DP>::kSmem,
           size_t(part_floats<R, DP>()) * sizeof(float)};
 }
 
 template <typename T, int WR, int DP>
 Variant shared_rows() {
   return {reinterpret_cast<const void*>(&paged_attn_rows_kernel<T, WR, DP>),
-          reinterpret_cast<const void*>(&paged_attn_join_kernel<T, WR * 16, DP>), WR * 16, WR * 64,
+          reinterpret_cast<const void*>(&paged_attn_join_kernel<T, WR * 16, DP>), WR * 16, WR * 64, true, sizeof(T),
           RowsShape<WR, DP>::kSmem, size_t(part_floats<WR * 16, DP>()) * sizeof(float)};
 }
 
@@ -1119,8 +1158,8 @@ template <typename T, int V, int DP>
 Variant fma_rows() {
   using Core = Fma<T, V, DP>;
   return {reinterpret_cast<const void*>(&paged_attn_fma_kernel<T, Core>),
-          reinterpret_cast<const void*>(&paged_attn_join_kernel<T, Core::kRows, DP>), Core::kRows, kThreads,
-          sizeof(Merge<Core::kRows, DP>), size_t(part_floats<Core::kRows, DP>()) * sizeof(float)};
+          reinterpret_cast<const void*>(&paged_attn_join_kernel<T, Core::kRows, DP>), Core::kRows, kThreads, false, sizeof(T),
+          sizeof(Merge<kWarps, Core::kRows, DP>), size_t(part_floats<Core::kRows, DP>()) * sizeof(float)};
 }
 
 // [bf16, f16] x ([8, 16 query rows] x [64, 128, 256 elements], [32, 48 rows] x [64, 128
@@ -1223,6 +1262,10 @@ cudaError_t plan_paged_attn(const AttnArgs& a, int dtype, int n_sm, AttnPlan* pl
 cudaError_t launch_paged_attn(const AttnArgs& args, const AttnPlan& plan, cudaStream_t s) {
   const Variant& k = variant_at(plan.variant);
   AttnArgs a = args;
+  // a negative scale turns the queries' signs (of two 16-bit elements) in the tensor-core variants
+  const size_t esz = k.esz;
+  a.wide_out = reinterpret_cast<uintptr_t>(a.out) % (4 * esz) == 0 && a.head_dim % 4 == 0;
+  if (k.tensor && a.scale_log2 < 0) a.scale_log2 = -a.scale_log2, a.q_sign = 0x80008000u;
   void* params[] = {&a};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(plan.n_workers));

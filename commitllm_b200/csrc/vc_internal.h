@@ -190,6 +190,8 @@ struct AttnArgs {
   int64_t cache_elems, row_span;
   const int32_t* seq_lens;     // [n_seqs]
   float scale_log2;            // scale * log2(e)
+  int32_t wide_out;            // four elements of out at a time
+  uint32_t q_sign;             // sign bits turned in pairs of query elements
   void* out;                   // [n_seqs][n_new][n_heads][head_dim]
   float* lse;                  // [n_seqs][n_new][n_heads] or nullptr
   float* parts;                // partial results of split units
