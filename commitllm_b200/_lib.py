@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(HERE, "libvcommit.so")
 VC_OK, VC_EINVAL, VC_ENOMEM, VC_ECUDA, VC_ETIMEDOUT, VC_ERANGE, VC_ENOTSUP = range(7)
 VC_DTYPE_BF16, VC_DTYPE_F32, VC_DTYPE_F64, VC_DTYPE_F16 = 0, 1, 2, 3
 VC_ROPE_NONE, VC_ROPE_LLAMA3, VC_ROPE_LINEAR = 0, 1, 2
+VC_CALL_ROPE_APPEND, VC_CALL_PAGED_ATTENTION, VC_CALL_VERIFY_TOKENS = 0, 1, 2
 
 SYMBOLS = (
     "vc_abi_version", "vc_last_error", "vc_ctx_create", "vc_ctx_destroy", "vc_ctx_sync",
@@ -24,7 +25,7 @@ SYMBOLS = (
     "vc_int_peak", "vc_wait_probe", "vc_kv_commit_noalloc", "vc_kv_open", "vc_io_extend", "vc_io_genesis",
     "vc_kv_transcript", "vc_kv_transcript_commit",
     "vc_rope_append", "vc_paged_attention", "vc_paged_attention_workspace",
-    "vc_verify_tokens", "vc_verify_tokens_workspace",
+    "vc_verify_tokens", "vc_verify_tokens_workspace", "vc_decode_call",
 )
 
 
@@ -123,6 +124,7 @@ def _declare(lib):
         "vc_verify_tokens": [P, c_int32, c_int32, c_int32, P, c_int32, c_int64, c_int64, P, c_int64, c_int64, P, P, P,
                              P, P, P, c_size_t],
         "vc_verify_tokens_workspace": [P, c_int32, c_int32, c_int32, POINTER(c_size_t)],
+        "vc_decode_call": [c_int32, c_int32, ctypes.c_char_p],
     }.items():
         fn = getattr(lib, name)
         fn.restype = c_int32

@@ -12,6 +12,7 @@
 #include <mutex>
 #include <string>
 #include <thread>
+#include <utility>
 #include <vector>
 
 #include "../../include/vcommit.h"
@@ -1301,6 +1302,49 @@ vc_status vc_verify_tokens(vc_ctx* c, int32_t n_seqs, int32_t n_draft, int32_t v
   const cudaError_t e = launch_verify(a, logits_dtype, c->n_sm, c->stream);
   if (e != cudaSuccess) return fail(VC_ECUDA, "vc_verify_tokens launch: %s", cudaGetErrorString(e));
   return VC_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+// One 64-bit slot as an argument of any declared type.
+struct Slot {
+  int64_t v;
+  template <typename T> operator T*() const { return reinterpret_cast<T*>(v); }
+  operator int32_t() const { return int32_t(v); }
+  operator int64_t() const { return v; }
+  operator size_t() const { return size_t(v); }
+  operator double() const {
+    double d;
+    std::memcpy(&d, &v, sizeof(d));
+    return d;
+  }
+};
+
+template <typename... A, size_t... I>
+vc_status call_slots(vc_status (*fn)(A...), const int64_t* s, std::index_sequence<I...>) {
+  return fn(static_cast<A>(Slot{s[I]})...);
+}
+
+template <typename... A>
+vc_status call_slots(vc_status (*fn)(A...), int32_t n, const int64_t* s) {
+  if (n != int32_t(sizeof...(A))) return fail(VC_EINVAL, "vc_decode_call: %d slots, %zu needed", n, sizeof...(A));
+  return call_slots(fn, s, std::index_sequence_for<A...>());
+}
+
+}  // namespace
+
+extern "C" {
+
+vc_status vc_decode_call(int32_t call, int32_t n_slots, const int64_t* slots) {
+  if (!slots) return fail(VC_EINVAL, "vc_decode_call: slots is NULL");
+  switch (call) {
+    case VC_CALL_ROPE_APPEND: return call_slots(vc_rope_append, n_slots, slots);
+    case VC_CALL_PAGED_ATTENTION: return call_slots(vc_paged_attention, n_slots, slots);
+    case VC_CALL_VERIFY_TOKENS: return call_slots(vc_verify_tokens, n_slots, slots);
+  }
+  return fail(VC_EINVAL, "vc_decode_call: no call %d", call);
 }
 
 vc_status vc_int_peak(vc_ctx* c, int32_t variant, int64_t iters, double* ops_per_s) {

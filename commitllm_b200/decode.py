@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -35,12 +36,40 @@ _CACHE_DTYPES = {torch.bfloat16: _lib.VC_DTYPE_BF16, torch.float16: _lib.VC_DTYP
                  torch.float32: _lib.VC_DTYPE_F32}
 
 
+# A decode step runs these calls layer by layer, often on a batch of one, where the
+# host's share of a call is longer than the GPU's.  So the arguments go over in one
+# packed buffer, each call tests everything in one expression, and looks for what to
+# complain about only when that fails.
+_ROPE = struct.Struct("21qdq")
+_ATTEND = struct.Struct("11qd4q")
+_VERIFY = struct.Struct("18q")
+_decode_call = None
+
+
+def _call(which: int, n: int, slots: bytes) -> None:
+    global _decode_call
+    if _decode_call is None:
+        _decode_call = lib().vc_decode_call
+    status = _decode_call(which, n, slots)
+    if status:
+        check(status)
+
+
+def _handle(ctx: Context) -> int:
+    return ctx._h.value or ctx.handle.value
+
+
 def _empty(ctx: Context, shape, dtype) -> torch.Tensor:
     # Context.empty without the stream switch when the stream is current already
-    if torch._C._cuda_getCurrentRawStream(ctx.device) == ctx.stream.cuda_stream \
-            and torch._C._cuda_getDevice() == ctx.device:
-        return torch.empty(shape, dtype=dtype, device="cuda")
+    if torch._C._cuda_getCurrentRawStream(ctx.device) == ctx.stream.cuda_stream:
+        return torch.empty(shape, dtype=dtype, device=ctx.stream.device)
     return ctx.empty(shape, dtype=dtype)
+
+
+def _empty_like(ctx: Context, t: torch.Tensor) -> torch.Tensor:
+    if torch._C._cuda_getCurrentRawStream(ctx.device) == ctx.stream.cuda_stream:
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
+    return ctx.empty(t.shape, dtype=t.dtype)
 
 
 def _on(ctx: Context, t: torch.Tensor, name: str) -> None:
@@ -50,8 +79,9 @@ def _on(ctx: Context, t: torch.Tensor, name: str) -> None:
 
 def _index(ctx: Context, t: torch.Tensor, name: str, shape) -> int:
     """Address of a contiguous int32 tensor of this shape."""
-    _on(ctx, t, name)
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == ctx.device and t.shape == shape
+            and t.is_contiguous()):
+        _on(ctx, t, name)
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)}")
     return t.data_ptr()
 
@@ -107,6 +137,7 @@ class PagedCache:
         d.v_layers = ctypes.cast(vp, ctypes.POINTER(ctypes.c_void_p))
         self.desc = d
         self._ref = ctypes.byref(d)
+        self._addr = ctypes.addressof(d)
         self._workspace = {}        # (n_new, n_heads) -> bytes
 
     def view(self, seq_lens: Sequence[int], layer_base: int = 0) -> KvCacheView:
@@ -227,26 +258,32 @@ def rope_append(cache: PagedCache, layer: int, q: torch.Tensor, k: torch.Tensor,
     ctx = cache.ctx
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
         raise ValueError("q must be [n_tokens, n_heads, head_dim]")
-    n, heads, dim = q.shape
-    _rows(ctx, q, "q", n, None, cache.head_dim, cache.dtype)
-    _rows(ctx, k, "k", n, cache.n_kv_heads, cache.head_dim, cache.dtype)
-    _rows(ctx, v, "v", n, cache.n_kv_heads, cache.head_dim, cache.dtype)
+    n, heads, _ = q.shape
+    dev, dt, dim = ctx.device, cache.dtype, cache.head_dim
+    kv = (n, cache.n_kv_heads, dim)
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if not (q.dtype is dt and k.dtype is dt and v.dtype is dt and q.shape[2] == dim and k.shape == kv and v.shape == kv
+            and qs[2] == 1 and ks[2] == 1 and vs[2] == 1 and q.get_device() == dev and k.get_device() == dev
+            and v.get_device() == dev):
+        _rows(ctx, q, "q", n, None, dim, dt)
+        _rows(ctx, k, "k", n, cache.n_kv_heads, dim, dt)
+        _rows(ctx, v, "v", n, cache.n_kv_heads, dim, dt)
     pos = _index(ctx, positions, "positions", (n,))
-    ids = None if seq_ids is None else _index(ctx, seq_ids, "seq_ids", (n,))
+    ids = 0 if seq_ids is None else _index(ctx, seq_ids, "seq_ids", (n,))
     inv = rope.inv_freq
-    _on(ctx, inv, "rope.inv_freq")
-    if inv.dtype != torch.float64 or not inv.is_contiguous():
-        raise ValueError("rope.inv_freq must be a contiguous float64 tensor")
+    if not (inv.dtype is torch.float64 and inv.get_device() == dev and inv.is_contiguous()):
+        raise ValueError(f"rope.inv_freq must be a contiguous float64 tensor on device {dev}")
     if q_out is None:
-        q_out = _empty(ctx, (n, heads, dim), cache.dtype)
+        q_out = _empty_like(ctx, q)
     else:
-        _rows(ctx, q_out, "q_out", n, heads, cache.head_dim, cache.dtype)
+        _rows(ctx, q_out, "q_out", n, heads, dim, dt)
     if n == 0:
         return q_out
-    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), q_out.stride()
-    check(lib().vc_rope_append(ctx.handle, cache._ref, layer, n, pos, ids, heads, q.data_ptr(), qs[0], qs[1],
-                               q_out.data_ptr(), os[0], os[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-                               inv.data_ptr(), 2 * inv.numel(), rope.factor, int(interleaved)))
+    os = q_out.stride()
+    _call(_lib.VC_CALL_ROPE_APPEND, 23,
+          _ROPE.pack(_handle(ctx), cache._addr, layer, n, pos, ids, heads, q.data_ptr(), qs[0], qs[1], q_out.data_ptr(),
+                     os[0], os[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], inv.data_ptr(),
+                     2 * inv.numel(), rope.factor, interleaved))
     return q_out
 
 
@@ -272,37 +309,41 @@ def paged_attention(cache: PagedCache, layer: int, q: torch.Tensor, seq_lens: to
     uses (new by default).
     """
     ctx = cache.ctx
-    _on(ctx, q, "q")
-    if q.dtype != cache.dtype or q.dim() != 4 or q.shape[3] != cache.head_dim:
-        raise ValueError(f"q must be {cache.dtype} [n_seqs, n_new, n_heads, {cache.head_dim}]")
+    if not isinstance(q, torch.Tensor) or q.dim() != 4:
+        raise ValueError("q must be [n_seqs, n_new, n_heads, head_dim]")
     S, N, H, D = q.shape
     qs = q.stride()
-    if qs[3] != 1:
-        raise ValueError("q must be contiguous within a head")
-    if S > cache.n_seqs:
-        raise ValueError(f"{S} sequences, the block table has {cache.n_seqs}")
-    if N < 1 or H < 1:
+    if not (q.dtype is cache.dtype and D == cache.head_dim and qs[3] == 1 and S <= cache.n_seqs and N > 0 and H > 0
+            and q.get_device() == ctx.device):
+        _on(ctx, q, "q")
+        if q.dtype != cache.dtype or D != cache.head_dim:
+            raise ValueError(f"q must be {cache.dtype} [n_seqs, n_new, n_heads, {cache.head_dim}]")
+        if qs[3] != 1:
+            raise ValueError("q must be contiguous within a head")
+        if S > cache.n_seqs:
+            raise ValueError(f"{S} sequences, the block table has {cache.n_seqs}")
         raise ValueError("n_new and n_heads must be at least 1")
     lens = _index(ctx, seq_lens, "seq_lens", (S,))
     if out is None:
-        out = _empty(ctx, (S, N, H, D), cache.dtype)
+        out = _empty_like(ctx, q)
     else:
         _on(ctx, out, "out")
         if out.dtype != cache.dtype or out.shape != q.shape or not out.is_contiguous():
             raise ValueError("out must be contiguous, of q's shape and dtype")
     lse = _empty(ctx, (S, N, H), torch.float32) if return_lse else None
-    need = cache.workspace_bytes(N, H)
+    need = cache._workspace.get((N, H)) or cache.workspace_bytes(N, H)
     if workspace is None:
         workspace = _empty(ctx, need, torch.uint8)
     else:
         _on(ctx, workspace, "workspace")
         if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
             raise ValueError("workspace must be a contiguous uint8 tensor")
+        need = workspace.numel()
     if S:
-        check(lib().vc_paged_attention(ctx.handle, cache._ref, layer, S, N, H, q.data_ptr(), qs[0], qs[1], qs[2], lens,
-                                       D ** -0.5 if scale is None else float(scale), out.data_ptr(),
-                                       None if lse is None else lse.data_ptr(), workspace.data_ptr(),
-                                       workspace.numel()))
+        _call(_lib.VC_CALL_PAGED_ATTENTION, 16,
+              _ATTEND.pack(_handle(ctx), cache._addr, layer, S, N, H, q.data_ptr(), qs[0], qs[1], qs[2], lens,
+                           D ** -0.5 if scale is None else scale, out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                           workspace.data_ptr(), need))
     return (out, lse) if return_lse else out
 
 
@@ -334,40 +375,44 @@ def verify_tokens(ctx: Context, logits: torch.Tensor, drafts: torch.Tensor, unif
     K/V rows stay in their pages until the next step writes them; commit with the
     lengths that ``counts`` gives.
     """
-    _on(ctx, logits, "logits")
-    if logits.dtype not in _CACHE_DTYPES or logits.dim() != 3 or 0 in logits.shape[1:]:
-        raise ValueError("logits must be float32, bfloat16 or float16 [n_seqs, n_draft + 1, vocab]")
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 3:
+        raise ValueError("logits must be [n_seqs, n_draft + 1, vocab]")
     S, N, V = logits.shape
     ls = logits.stride()
-    if ls[2] != 1 and V > 1:
-        raise ValueError("logits must be contiguous within a row")
+    dev = ctx.device
+    if not (logits.dtype in _CACHE_DTYPES and N > 0 and V > 0 and (ls[2] == 1 or V == 1) and logits.get_device() == dev):
+        _on(ctx, logits, "logits")
+        raise ValueError("logits must be float32, bfloat16 or float16 [n_seqs, n_draft + 1, vocab], contiguous within a row")
     x = _index(ctx, drafts, "drafts", (S, N - 1))
-    _on(ctx, uniforms, "uniforms")
-    if uniforms.dtype != torch.float64 or uniforms.shape != (S, N) or not uniforms.is_contiguous():
-        raise ValueError(f"uniforms must be contiguous float64 [{S}, {N}]")
-    _on(ctx, temperature, "temperature")
-    if temperature.dtype != torch.float32 or temperature.shape != (S,) or not temperature.is_contiguous():
-        raise ValueError(f"temperature must be contiguous float32 [{S}]")
-    probs, ps = None, (0, 0)
+    if not (uniforms.dtype is torch.float64 and uniforms.shape == (S, N) and uniforms.get_device() == dev
+            and uniforms.is_contiguous()):
+        raise ValueError(f"uniforms must be contiguous float64 [{S}, {N}] on device {dev}")
+    if not (temperature.dtype is torch.float32 and temperature.shape == (S,) and temperature.get_device() == dev
+            and temperature.is_contiguous()):
+        raise ValueError(f"temperature must be contiguous float32 [{S}] on device {dev}")
+    probs, ps = 0, (0, 0)
     if draft_probs is not None:
-        _on(ctx, draft_probs, "draft_probs")
         ps = draft_probs.stride()
-        if draft_probs.dtype != torch.float32 or draft_probs.shape != (S, N - 1, V) or (ps[2] != 1 and V > 1):
-            raise ValueError(f"draft_probs must be float32 [{S}, {N - 1}, {V}], contiguous within a row")
+        if not (draft_probs.dtype is torch.float32 and draft_probs.shape == (S, N - 1, V) and (ps[2] == 1 or V == 1)
+                and draft_probs.get_device() == dev):
+            raise ValueError(f"draft_probs must be float32 [{S}, {N - 1}, {V}] on device {dev}, contiguous within a row")
         probs = draft_probs.data_ptr()
     tokens = _empty(ctx, (S, N), torch.int32)
     counts = _empty(ctx, (S,), torch.int32)
     if S == 0:
         return tokens, counts
     if workspace is None:
-        need = ctypes.c_size_t()
-        check(lib().vc_verify_tokens_workspace(ctx.handle, S, N - 1, V, ctypes.byref(need)))
-        workspace = _empty(ctx, need.value, torch.uint8)
+        size = ctypes.c_size_t()
+        check(lib().vc_verify_tokens_workspace(ctx.handle, S, N - 1, V, ctypes.byref(size)))
+        need = size.value
+        workspace = _empty(ctx, need, torch.uint8)
     else:
         _on(ctx, workspace, "workspace")
         if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
             raise ValueError("workspace must be a contiguous uint8 tensor")
-    check(lib().vc_verify_tokens(ctx.handle, S, N - 1, V, logits.data_ptr(), _CACHE_DTYPES[logits.dtype], ls[0], ls[1],
-                                 probs or None, ps[0], ps[1], x, uniforms.data_ptr(), temperature.data_ptr(),
-                                 tokens.data_ptr(), counts.data_ptr(), workspace.data_ptr(), workspace.numel()))
+        need = workspace.numel()
+    _call(_lib.VC_CALL_VERIFY_TOKENS, 18,
+          _VERIFY.pack(_handle(ctx), S, N - 1, V, logits.data_ptr(), _CACHE_DTYPES[logits.dtype], ls[0], ls[1], probs, ps[0],
+                       ps[1], x, uniforms.data_ptr(), temperature.data_ptr(), tokens.data_ptr(), counts.data_ptr(),
+                       workspace.data_ptr(), need))
     return tokens, counts

@@ -54,4 +54,8 @@ def test_entry_points_refuse_null_arguments():
     assert lib.vc_paged_attention_workspace(None, None, 0, 0, ctypes.byref(out)) == _lib.VC_EINVAL
     assert lib.vc_verify_tokens(None, 0, 0, 0, None, 0, 0, 0, None, 0, 0, None, None, None, None, None, None,
                                 0) == _lib.VC_EINVAL
+    assert lib.vc_decode_call(0, 23, None) == _lib.VC_EINVAL
+    assert lib.vc_decode_call(3, 0, b"") == _lib.VC_EINVAL
+    assert lib.vc_decode_call(1, 15, bytes(120)) == _lib.VC_EINVAL
+    assert lib.vc_decode_call(1, 16, bytes(128)) == _lib.VC_EINVAL
     assert lib.vc_verify_tokens_workspace(None, 0, 0, 0, ctypes.byref(out)) == _lib.VC_EINVAL
