@@ -191,6 +191,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Weights are taken relative to a reference that is at most 2^8 below the largest one
+// seen: it follows the maximum only when that has grown by more, so the sums so far are
+// seldom rescaled (a maximum of random scores grows in half of the first 30 tiles) and
+// no weight passes 2^8, which f16 holds too.
+constexpr float kSlack = 8.f;
+
 // Shared memory of a unit's end: the outputs of R rows from W warps that saw different
 // keys, D elements at a time, with their maxima (base-2 exponents) and sums.  Rows are
 // padded by 16 bytes: a warp's stores then fall into different banks.
@@ -374,12 +380,6 @@ __device__ __forceinline__ void pv_of_token(float (&o)[4], const uint32_t (&vf)[
   if (c0) o[0] = y[0], o[2] = y[2];
   if (c1) o[1] = y[1], o[3] = y[3];
 }
-
-// Weights are taken relative to a reference that is at most 2^8 below the largest one
-// seen: it follows the maximum only when that has grown by more, so the sums so far are
-// seldom rescaled (a maximum of random scores grows in half of the first 30 tiles) and
-// no weight passes 2^8, which f16 holds too.
-constexpr float kSlack = 8.f;
 
 // Scores to weights for one column tile of 8 query rows (the lane's: lane / 4) and NB
 // blocks of 16 keys (the lane's of block b: 16b + 2c + {0, 1, 8, 9}; those from `left`
@@ -939,9 +939,12 @@ struct Fma {
     int p = t0 * kTile + warp * 16 + (lane >> 3);
     int64_t off = p < len ? row_of(a, seq, p) : -1;
     load(kx, kb + off, off >= 0, a.head_dim);
+    load(vx, vb + off, off >= 0, a.head_dim);
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
-      load(vx, vb + off, off >= 0, a.head_dim);
+      // the next four keys' rows are found now, and loaded as soon as this step's are used
+      const int pn = (i & 3) == 3 ? p + kTile - 12 : p + 4;
+      const int64_t offn = i + 1 < n && pn < len ? row_of(a, seq, pn) : -1;
       float s[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) s[r] = 0.f;
@@ -951,9 +954,6 @@ struct Fma {
         for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int j = 0; j < V; ++j) s[r] = fmaf(qs[r][(e * 8 + g) * V + j], kx[e * V + j], s[r]);
-      // the next four keys
-      const int pn = (i & 3) == 3 ? p + kTile - 12 : p + 4;
-      const int64_t offn = i + 1 < n && pn < len ? row_of(a, seq, pn) : -1;
       load(kx, kb + offn, offn >= 0, a.head_dim);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -961,18 +961,24 @@ struct Fma {
         for (int d = 1; d < 8; d <<= 1) s[r] += __shfl_xor_sync(~0u, s[r], d);
         const bool seen = p < lim[r];
         const float x = seen ? s[r] * a.scale_log2 : ninf();
-        // the eight lanes of a key keep their own maximum: keys of other lane groups join at the end
-        const float top = fmaxf(m[r], x);
-        const float ref = top == ninf() ? 0.f : top;
-        const float f = exp2f(m[r] - ref);
-        const float e = exp2f(x - ref);
-        m[r] = top;
-        l[r] = fmaf(l[r], f, e);
+        // the eight lanes of a key keep their own reference: the other keys' lanes join at the end
+        if (__any_sync(~0u, x > m[r] + kSlack)) {
+          const float top = fmaxf(m[r], x);
+          const float f = m[r] == ninf() ? 0.f : ex2(m[r] - top);
+          l[r] *= f;
+#pragma unroll
+          for (int j = 0; j < NL * V; ++j) o[r][j] *= f;
+          m[r] = top;
+        }
+        const float ref = m[r] == ninf() ? 0.f : m[r];
+        const float e = ex2(x - ref);
+        l[r] += e;
         if (seen) {
 #pragma unroll
-          for (int j = 0; j < NL * V; ++j) o[r][j] = fmaf(e, vx[j], o[r][j] * f);
+          for (int j = 0; j < NL * V; ++j) o[r][j] = fmaf(e, vx[j], o[r][j]);
         }
       }
+      load(vx, vb + offn, offn >= 0, a.head_dim);
       p = pn;
       off = offn;
     }
@@ -985,7 +991,7 @@ struct Fma {
       float top = fmaxf(m[r], __shfl_xor_sync(~0u, m[r], 8));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
       const float ref = top == ninf() ? 0.f : top;
-      const float f = exp2f(m[r] - ref);
+      const float f = ex2(m[r] - ref);
       float sum = l[r] * f;
       sum += __shfl_xor_sync(~0u, sum, 8);
       sum += __shfl_xor_sync(~0u, sum, 16);
@@ -1103,7 +1109,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __g
   for (int64_t w = wa + warp; w <= wb; w += kWarps) {
     const float* src = part(w);
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + R * DP + 2 * r));
-    const float f = exp2f(ml.x - ref);
+    const float f = ex2(ml.x - ref);
     l += f * ml.y;
 #pragma unroll
     for (int i = 0; i < kQ; ++i) {

@@ -23,7 +23,7 @@
 namespace vc {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 template <typename T> __device__ __forceinline__ float to_f32(T x);
 template <> __device__ __forceinline__ float to_f32<float>(float x) { return x; }
