@@ -233,13 +233,16 @@ struct Weights {
     const double w = pow2((double(x) - m) * c, table);
     return x < none ? 0.0 : w;
   }
+  template <bool kOver>
   __device__ __forceinline__ double of(float x, float qv) const {
     const double w = plain(x);
-    if (!q) return w;
+    if (!kOver) return w;
     const double d = fma(w, scale, -double(qv));
     return d > 0.0 ? d : 0.0;
   }
-  __device__ __forceinline__ double at(int v) const { return of(to_f32(l[v]), q ? q[v] : 0.f); }
+  __device__ __forceinline__ double at(int v) const {
+    return q ? of<true>(to_f32(l[v]), q[v]) : of<false>(to_f32(l[v]), 0.f);
+  }
 };
 
 // This CTA's slice [lo, hi) of the vocabulary; its warps hold equal contiguous
@@ -255,37 +258,55 @@ struct Box {
   int token;
 };
 
-// Sum of the weights over the slice: all threads get the CTA's, box.warp keeps the parts.
-template <typename T>
-__device__ double slice_sum(const Weights<T>& w, const Slice& sl, Box& box) {
+// Sum of the weights over a warp's part [b, e), by its lanes; kOver: over the draft's
+// probabilities.
+template <typename T, bool kOver>
+__device__ __forceinline__ double part_sum(const Weights<T>& w, int b, int e) {
   constexpr int N = 16 / sizeof(T);
+  constexpr int kBatch = sizeof(T) == 4 ? 2 : 1;      // chunks a lane has under way
   struct alignas(16) Chunk {
     T v[N];
   };
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int b = min(sl.lo + warp * sl.per_warp, sl.hi), e = min(b + sl.per_warp, sl.hi);
+  const int lane = threadIdx.x & 31;
   double v = 0;
   int j = b;
   if (w.wide) {
     const int n = (e - b) / N;
-#pragma unroll (16 / N)
-    for (int k = lane; k < n; k += 32) {
-      const Chunk ch = *reinterpret_cast<const Chunk*>(w.l + b + k * N);
-      float qv[N] = {};
-      if (w.q) {
+    for (int k = lane; k < n; k += 32 * kBatch) {
+      Chunk ch[kBatch];
+      float qv[kBatch * N];
 #pragma unroll
-        for (int i = 0; i < N; i += 4)
-          *reinterpret_cast<float4*>(qv + i) = *reinterpret_cast<const float4*>(w.q + b + k * N + i);
+      for (int x = 0; x < kBatch; ++x) {
+        if (k + 32 * x >= n) continue;
+        ch[x] = *reinterpret_cast<const Chunk*>(w.l + b + (k + 32 * x) * N);
+        if (kOver) {
+#pragma unroll
+          for (int i = 0; i < N; i += 4)
+            *reinterpret_cast<float4*>(qv + x * N + i) = *reinterpret_cast<const float4*>(w.q + b + (k + 32 * x) * N + i);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < N; ++i) v += w.of(to_f32(ch.v[i]), qv[i]);
+      for (int x = 0; x < kBatch; ++x) {
+        if (k + 32 * x >= n) continue;
+#pragma unroll
+        for (int i = 0; i < N; ++i) v += w.template of<kOver>(to_f32(ch[x].v[i]), kOver ? qv[x * N + i] : 0.f);
+      }
     }
     j = b + n * N;
   }
 #pragma unroll 4
-  for (j += lane; j < e; j += 32) v += w.at(j);
+  for (j += lane; j < e; j += 32) v += w.template of<kOver>(to_f32(w.l[j]), kOver ? w.q[j] : 0.f);
 #pragma unroll
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+  return v;
+}
+
+// Sum of the weights over the slice: all threads get the CTA's, box.warp keeps the parts.
+template <typename T>
+__device__ double slice_sum(const Weights<T>& w, const Slice& sl, Box& box) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = min(sl.lo + warp * sl.per_warp, sl.hi), e = min(b + sl.per_warp, sl.hi);
+  const double v = w.q ? part_sum<T, true>(w, b, e) : part_sum<T, false>(w, b, e);
   __syncthreads();               // the last call's parts have been read
   if (lane == 0) box.warp[warp] = v;
   __syncthreads();
