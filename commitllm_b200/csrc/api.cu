@@ -1257,7 +1257,7 @@ static vc_status plan_verify_call(vc_ctx* c, int32_t n_seqs, int32_t n_draft, in
   *bytes = 0;
   if (n_seqs == 0) return VC_OK;
   plan_verify(a, c->n_sm);
-  *bytes = size_t(n_seqs) * size_t(n_draft + 1) * size_t(a->splits) * sizeof(VerifyPart);
+  *bytes = size_t(n_seqs) * size_t(n_draft + 1) * kVerifyRowBytes;
   return VC_OK;
 }
 

@@ -214,6 +214,7 @@ struct VerifyPart {            // one slice of a logits row
   float m;                     // maximum
   int32_t best;                // its lowest index
 };
+constexpr size_t kVerifyRowBytes = 1024;      // workspace of a logits row: up to 32 slices
 struct VerifyArgs {
   int32_t n_seqs, n_draft, vocab;
   const void* logits; int64_t logits_seq, logits_tok;          // elements

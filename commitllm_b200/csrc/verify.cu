@@ -33,6 +33,7 @@ constexpr int kStatThreads = 256;
 constexpr int kPickThreads = 512;
 constexpr int kPickWarps = kPickThreads / 32;
 constexpr int kMaxCluster = 8;
+static_assert(32 * sizeof(VerifyPart) <= kVerifyRowBytes, "a row's slices fit its workspace");
 
 // How far a keep-or-refuse quantity of the f32 sums may be from its exact value,
 // relative to the row's sum: an exponent of at most 126 (smaller weights are
@@ -108,15 +109,28 @@ __device__ __forceinline__ void stat_slice(const T* src, int lo, int hi, float c
     const float l[1] = {to_f32(src[lo + threadIdx.x])};
     r.template add<1, 1>(l, lo + threadIdx.x, 0, c, x);
   }
+  // a batch of chunks; of f32 ones, the next is on its way while one is summed (74.6 ->
+  // 71.7 us for 320 rows; of 16-bit ones it costs too many registers: 39 -> 48 us)
   int j = threadIdx.x;
-  for (; j + (kBatch - 1) * kStatThreads < body; j += kBatch * kStatThreads) {
-    const int at = lo + head + j * N;
-    Chunk ch[kBatch];
+  constexpr bool kAhead = sizeof(T) == 4;
+  constexpr int kStep = kBatch * kStatThreads;
+  Chunk ch[kBatch];
+  auto load = [&](int from) {
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) ch[k] = *reinterpret_cast<const Chunk*>(src + at + k * kStatThreads * N);
+    for (int k = 0; k < kBatch; ++k)
+      ch[k] = *reinterpret_cast<const Chunk*>(src + lo + head + (from + k * kStatThreads) * N);
+  };
+  bool full = j + kStep - kStatThreads < body;
+  if (kAhead && full) load(j);
+  while (full) {
+    if (!kAhead) load(j);
     float l[kBatch * N];
 #pragma unroll
     for (int e = 0; e < kBatch * N; ++e) l[e] = to_f32(ch[e / N].v[e % N]);
+    const int at = lo + head + j * N;
+    j += kStep;
+    full = j + kStep - kStatThreads < body;
+    if (kAhead && full) load(j);
     r.template add<kBatch * N, N>(l, at, kStatThreads * N, c, x);
   }
   for (; j < body; j += kStatThreads) {
@@ -272,24 +286,38 @@ __device__ __forceinline__ double part_sum(const Weights<T>& w, int b, int e) {
   int j = b;
   if (w.wide) {
     const int n = (e - b) / N;
-    for (int k = lane; k < n; k += 32 * kBatch) {
-      Chunk ch[kBatch];
-      float qv[kBatch * N];
+    // chunks past the end are read again and not counted, so a batch has no branches
+    Chunk ch[kBatch];
+    float4 qv[kBatch * N / 4];
+    auto load = [&](int k) {
 #pragma unroll
       for (int x = 0; x < kBatch; ++x) {
-        if (k + 32 * x >= n) continue;
-        ch[x] = *reinterpret_cast<const Chunk*>(w.l + b + (k + 32 * x) * N);
+        const int at = b + min(k + 32 * x, n - 1) * N;
+        ch[x] = *reinterpret_cast<const Chunk*>(w.l + at);
         if (kOver) {
 #pragma unroll
-          for (int i = 0; i < N; i += 4)
-            *reinterpret_cast<float4*>(qv + x * N + i) = *reinterpret_cast<const float4*>(w.q + b + (k + 32 * x) * N + i);
+          for (int i = 0; i < N / 4; ++i) qv[x * (N / 4) + i] = *reinterpret_cast<const float4*>(w.q + at + 4 * i);
         }
       }
+    };
+    if (n > 0) load(lane);
+    for (int k = lane; k - lane < n; k += 32 * kBatch) {
+      float l[kBatch * N], q[kBatch * N];
+#pragma unroll
+      for (int x = 0; x < kBatch; ++x)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          l[x * N + i] = to_f32(ch[x].v[i]);
+          const float4 f = qv[x * (N / 4) + i / 4];
+          q[x * N + i] = !kOver ? 0.f : i % 4 == 0 ? f.x : i % 4 == 1 ? f.y : i % 4 == 2 ? f.z : f.w;
+        }
+      if (k - lane + 32 * kBatch < n) load(k + 32 * kBatch);      // while this batch is weighed
 #pragma unroll
       for (int x = 0; x < kBatch; ++x) {
-        if (k + 32 * x >= n) continue;
+        double t = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) v += w.template of<kOver>(to_f32(ch[x].v[i]), kOver ? qv[x * N + i] : 0.f);
+        for (int i = 0; i < N; ++i) t += w.template of<kOver>(l[x * N + i], q[x * N + i]);
+        v += k + 32 * x < n ? t : 0.0;
       }
     }
     j = b + n * N;
@@ -374,7 +402,7 @@ __device__ void find(const Weights<T>& w, const Slice& sl, Box& box, const doubl
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kPickThreads, 2) verify_pick_kernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(kPickThreads, 1) verify_pick_kernel(const __grid_constant__ VerifyArgs a) {
   __shared__ Box box;
   __shared__ Row rows[kPickWarps];
   __shared__ double table[kTable];
@@ -586,10 +614,10 @@ void plan_verify(VerifyArgs* a, int n_sm) {
 }
 
 cudaError_t launch_verify(const VerifyArgs& a, int dtype, int n_sm, cudaStream_t s) {
-  // CTAs of a sequence's cluster: as many as stay resident at once (two an SM), one
-  // for a short row
+  // CTAs of a sequence's cluster: as many as stay resident at once (one an SM, whose
+  // 128 registers a thread measured 3 % faster than two with 64), one for a short row
   int cluster = a.vocab > 4096 ? kMaxCluster : 1;
-  while (cluster > 1 && int64_t(a.n_seqs) * cluster > 2 * n_sm) cluster /= 2;
+  while (cluster > 1 && int64_t(a.n_seqs) * cluster > n_sm) cluster /= 2;
   switch (dtype) {
     case 0: return launch_t<__nv_bfloat16>(a, cluster, s);
     case 1: return launch_t<float>(a, cluster, s);

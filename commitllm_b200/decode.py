@@ -43,6 +43,7 @@ _CACHE_DTYPES = {torch.bfloat16: _lib.VC_DTYPE_BF16, torch.float16: _lib.VC_DTYP
 _ROPE = struct.Struct("21qdq")
 _ATTEND = struct.Struct("11qd4q")
 _VERIFY = struct.Struct("18q")
+_VERIFY_ROW_BYTES = 1024        # vc_verify_tokens_workspace: this many for each logits row
 _decode_call = None
 
 
@@ -402,9 +403,7 @@ def verify_tokens(ctx: Context, logits: torch.Tensor, drafts: torch.Tensor, unif
     if S == 0:
         return tokens, counts
     if workspace is None:
-        size = ctypes.c_size_t()
-        check(lib().vc_verify_tokens_workspace(ctx.handle, S, N - 1, V, ctypes.byref(size)))
-        need = size.value
+        need = S * N * _VERIFY_ROW_BYTES
         workspace = _empty(ctx, need, torch.uint8)
     else:
         _on(ctx, workspace, "workspace")
