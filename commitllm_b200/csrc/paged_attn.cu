@@ -879,11 +879,11 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
   }
 }
 
-// ---------------------------- f32 rows, and 16-bit rows of any alignment: FMAs
+// ----------------------------------------------- rows of any alignment: FMAs
 
 // Eight lanes share a key (four keys at a time, 16 per warp and tile); each holds
 // DP / 8 of its elements.  V elements a load; element (i, e) of lane g is
-// (i * 8 + g) * V + e.  The query rows sit in shared memory as f32, scaled.
+// (i * 8 + g) * V + e.  The query rows sit in shared memory as f32.
 template <typename T, int V, int DP>
 struct Fma {
   static constexpr int R = 4;
@@ -1045,6 +1045,217 @@ __global__ void __launch_bounds__(kThreads) paged_attn_fma_kernel(const __grid_c
   }
 }
 
+// f32 rows on 16-byte boundaries: the ring of paged_attn_tc_kernel in stages of 8 keys,
+// with the products in f32 FMAs (512 a lane for 8 keys and 8 query rows, under half of
+// what a SM does while it loads those keys).  Eight lanes share a key, four keys at a
+// time; a lane's elements of a row are chunks i * 8 + lane % 8 of four.  The first
+// version loaded straight into registers, one step ahead: 4.0 TB/s, 26 us for a call of
+// 20 MB that spends most of its time on the way from load to load.
+template <int R, int DP>
+struct F32Shape {
+  static constexpr int kKeys = 8;
+  static constexpr int kStage = kKeys * DP * 4 * 2;
+  static constexpr int kStages = DP == 64 ? 6 : 3;
+  static constexpr int kRing = kWarps * kStages * kStage;
+  using Mg = Merge<kWarps, R, DP>;
+  static constexpr size_t kSmem = kRing + sizeof(Mg);
+};
+
+template <int R, int DP>
+__global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_f32_kernel(const __grid_constant__ AttnArgs a) {
+  using Shape = F32Shape<R, DP>;
+  constexpr int NL = DP / 32;          // four-element chunks a lane has of a row
+  constexpr int kStages = Shape::kStages;
+  constexpr int kCols = DP / 4;        // 16-byte chunks of a row
+  extern __shared__ __align__(128) char smem[];
+  typename Shape::Mg& mg = *reinterpret_cast<typename Shape::Mg*>(smem + Shape::kRing);
+  float(*qs)[DP + 4] = mg.o[0];        // the queries sit where the outputs will
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane & 7, kq = lane >> 3;
+  char* ring = smem + warp * (kStages * Shape::kStage);
+  const uint32_t ring_s = smem_addr(ring);
+  const int row_tiles = (a.rows + R - 1) / R;
+  const int units = a.n_kv_heads * row_tiles;
+  const int range = blockIdx.x / units, unit = blockIdx.x - range * units;
+  const int rt = unit / a.n_kv_heads, kvh = unit - rt * a.n_kv_heads, row0 = rt * R;
+  const Place pl = locate<kWarps>(a, range);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t chunk = chunk_of(pl.total, a.n_ranges);
+  const int64_t begin = int64_t(range) * chunk;
+  const int64_t end = begin + chunk < pl.total ? begin + chunk : pl.total;
+  if (begin >= end) return;
+  float* parts = a.parts + int64_t(blockIdx.x) * 2 * part_floats<R, DP>();
+
+  // ---- loading: lane i < 8 finds key i's row, one stage before it is copied
+  Cursor ahead;
+  ahead.at(a, pl.seq, pl.seq_base);
+  int64_t next = begin;                // tile, and which 8 of the warp's 16 keys of it
+  int next_half = 0;
+  int page = 0, slot = 0;
+  bool real = false;
+  auto look = [&]() {
+    real = false;
+    const int64_t t = ahead.advance(a, next, end);
+    if (t != next) next = t, next_half = 0;
+    if (next < end) {
+      const int p = int(next - ahead.base) * kTile + warp * 16 + next_half * 8 + lane;
+      if (lane < 8 && p < ahead.len) {
+        const int block = unsigned(p) / unsigned(a.block_size);
+        page = __ldg(a.block_tables + int64_t(ahead.seq) * a.max_blocks + block);
+        slot = p - block * a.block_size;
+        real = true;
+      }
+    }
+  };
+  int fill = 0;
+  auto issue = [&]() {
+    if (next < end) {
+      int64_t off = -1;
+      if (real) {
+        off = int64_t(page) * a.stride_page + int64_t(slot) * a.stride_row;
+        if (page < 0 || off + a.row_span > a.cache_elems) {
+          *a.err = 1;
+          off = -1;
+        } else {
+          off += kvh * a.stride_head;
+        }
+      }
+      if (next_half) ++next;
+      next_half ^= 1;
+      look();
+      const uint32_t dst = ring_s + fill * Shape::kStage;
+#pragma unroll
+      for (int j = 0; j < 8 * kCols / 32; ++j) {
+        const int row = (j * 32 + lane) / kCols, col = (j * 32 + lane) % kCols;
+        const int64_t o = __shfl_sync(~0u, off, row);
+        const int size = o >= 0 && col * 4 < a.head_dim ? 16 : 0;
+        const int64_t at = size ? o + col * 4 : 0;
+        const uint32_t d = dst + (row * kCols + col) * 16;
+        copy16(d, static_cast<const float*>(a.k) + at, size);
+        copy16(d + 8 * DP * 4, static_cast<const float*>(a.v) + at, size);
+      }
+    }
+    fill = fill + 1 == kStages ? 0 : fill + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  look();
+  for (int i = 0; i < kStages - 1; ++i) issue();
+
+  float4 o[R][NL];
+  float m[R], l[R];
+  int lim[R];
+  int use = 0;
+  Cursor now;
+  now.at(a, pl.seq, pl.seq_base);
+  int64_t cur = begin;
+  while ((cur = now.advance(a, cur, end)) < end) {
+    const int seq = now.seq, len = now.len;
+    const int t0 = int(cur - now.base);
+    const int t1 = now.nt - t0 < end - cur ? now.nt : t0 + int(end - cur);
+    for (int i = threadIdx.x; i < R * DP; i += kThreads) {
+      const int r = i / DP, d = i - r * DP;
+      qs[r][d] = row0 + r < a.rows && d < a.head_dim ? static_cast<const float*>(a.q)[row_at(a, seq, kvh, row0 + r).q + d] : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      lim[r] = row0 + r < a.rows ? len - a.n_new + 1 + row_at(a, seq, kvh, row0 + r).tok : 0;
+      m[r] = ninf();
+      l[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) o[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    __syncthreads();
+    const int sure = len - a.n_new + 1;
+#pragma unroll 1
+    for (int step = t0 * 2; step < t1 * 2; ++step) {
+      const int p0 = (step >> 1) * kTile + warp * 16 + (step & 1) * 8;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncwarp();                    // the stage has landed for all lanes, and the one before is free
+      issue();
+      const float4* kst = reinterpret_cast<const float4*>(ring + use * Shape::kStage);
+      const float4* vst = kst + 8 * kCols;
+      use = use + 1 == kStages ? 0 : use + 1;
+      // the lane's keys: kq and kq + 4
+      float s[R][2];
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[r][0] = s[r][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const float4 k0 = kst[kq * kCols + i * 8 + g], k1 = kst[(kq + 4) * kCols + i * 8 + g];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float4 x = *reinterpret_cast<const float4*>(&qs[r][(i * 8 + g) * 4]);
+          s[r][0] = fmaf(x.x, k0.x, fmaf(x.y, k0.y, fmaf(x.z, k0.z, fmaf(x.w, k0.w, s[r][0]))));
+          s[r][1] = fmaf(x.x, k1.x, fmaf(x.y, k1.y, fmaf(x.z, k1.z, fmaf(x.w, k1.w, s[r][1]))));
+        }
+      }
+      const bool all_seen = p0 + 8 <= sure;
+      float e[R][2];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+          for (int d = 1; d < 8; d <<= 1) s[r][x] += __shfl_xor_sync(~0u, s[r][x], d);
+          s[r][x] = all_seen || p0 + kq + 4 * x < lim[r] ? s[r][x] * a.scale_log2 : ninf();
+        }
+        // the eight lanes of a key keep their own reference: the other lanes' join at the end
+        const float top = fmaxf(s[r][0], s[r][1]);
+        if (__any_sync(~0u, top > m[r] + kSlack)) {
+          const float to = fmaxf(m[r], top);
+          const float f = m[r] == ninf() ? 0.f : ex2(m[r] - to);
+          l[r] *= f;
+#pragma unroll
+          for (int i = 0; i < NL; ++i) o[r][i].x *= f, o[r][i].y *= f, o[r][i].z *= f, o[r][i].w *= f;
+          m[r] = to;
+        }
+        const float ref = m[r] == ninf() ? 0.f : m[r];
+        e[r][0] = ex2(s[r][0] - ref), e[r][1] = ex2(s[r][1] - ref);
+        l[r] += e[r][0] + e[r][1];
+      }
+      // a value that a row does not see must not reach it, not even times 0
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          const float4 v = vst[(kq + 4 * x) * kCols + i * 8 + g];
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (all_seen || p0 + kq + 4 * x < lim[r]) {
+              o[r][i].x = fmaf(e[r][x], v.x, o[r][i].x);
+              o[r][i].y = fmaf(e[r][x], v.y, o[r][i].y);
+              o[r][i].z = fmaf(e[r][x], v.z, o[r][i].z);
+              o[r][i].w = fmaf(e[r][x], v.w, o[r][i].w);
+            }
+        }
+      }
+    }
+    __syncthreads();                   // the queries make place
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = fmaxf(m[r], __shfl_xor_sync(~0u, m[r], 8));
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+      const float f = ex2(m[r] - (top == ninf() ? 0.f : top));
+      float sum = l[r] * f;
+      sum += __shfl_xor_sync(~0u, sum, 8);
+      sum += __shfl_xor_sync(~0u, sum, 16);
+      if (lane == 0) mg.m[warp][r] = top, mg.l[warp][r] = sum;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        float y[4] = {o[r][i].x * f, o[r][i].y * f, o[r][i].z * f, o[r][i].w * f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          y[j] += __shfl_xor_sync(~0u, y[j], 8);
+          y[j] += __shfl_xor_sync(~0u, y[j], 16);
+        }
+        if (lane < 8) *reinterpret_cast<float4*>(&mg.o[warp][r][(i * 8 + g) * 4]) = make_float4(y[0], y[1], y[2], y[3]);
+      }
+    }
+    float* part = parts + (t0 == 0 ? part_floats<R, DP>() : 0);
+    emit<float, kWarps, R, DP, DP>(a, mg, {seq, kvh, row0, t0 == 0 && t1 == now.nt ? nullptr : part, part + R * DP}, 8, true, 0);
+    cur += t1 - t0;
+  }
+}
+
 // One query row: the parts of its sequence joined in the ranges' order; sequences
 // in one range are done, those without a key get zeros.
 template <typename T, int R, int DP>
@@ -1160,6 +1371,13 @@ Variant shared_rows() {
           RowsShape<WR, DP>::kSmem, size_t(part_floats<WR * 16, DP>()) * sizeof(float)};
 }
 
+template <int R, int DP>
+Variant f32_rows() {
+  return {reinterpret_cast<const void*>(&paged_attn_f32_kernel<R, DP>),
+          reinterpret_cast<const void*>(&paged_attn_join_kernel<float, R, DP>), R, kThreads, false, sizeof(float),
+          F32Shape<R, DP>::kSmem, size_t(part_floats<R, DP>()) * sizeof(float)};
+}
+
 template <typename T, int V, int DP>
 Variant fma_rows() {
   using Core = Fma<T, V, DP>;
@@ -1169,8 +1387,8 @@ Variant fma_rows() {
 }
 
 // [bf16, f16] x ([8, 16 query rows] x [64, 128, 256 elements], [32, 48 rows] x [64, 128
-// elements]), then f32 and the 16-bit types of any alignment.
-constexpr int kVariants = 28;
+// elements]), then f32, and f32 and the 16-bit types of any alignment.
+constexpr int kVariants = 31;
 template <typename T>
 struct TcVariants {
   static void fill(Variant* v) {
@@ -1187,10 +1405,11 @@ struct Variants {
     using hf = __half;
     TcVariants<bf>::fill(v);
     TcVariants<hf>::fill(v + 10);
-    v[20] = fma_rows<float, 4, 128>(), v[21] = fma_rows<float, 4, 256>();
-    v[22] = fma_rows<float, 1, 128>(), v[23] = fma_rows<float, 1, 256>();
-    v[24] = fma_rows<bf, 1, 128>(), v[25] = fma_rows<bf, 1, 256>();
-    v[26] = fma_rows<hf, 1, 128>(), v[27] = fma_rows<hf, 1, 256>();
+    v[20] = f32_rows<4, 64>(), v[21] = f32_rows<4, 128>(), v[22] = f32_rows<4, 256>();
+    v[23] = f32_rows<8, 64>(), v[24] = f32_rows<8, 128>();
+    v[25] = fma_rows<float, 1, 128>(), v[26] = fma_rows<float, 1, 256>();
+    v[27] = fma_rows<bf, 1, 128>(), v[28] = fma_rows<bf, 1, 256>();
+    v[29] = fma_rows<hf, 1, 128>(), v[30] = fma_rows<hf, 1, 256>();
   }
 };
 const Variant& variant_at(int i) {
@@ -1231,15 +1450,14 @@ cudaError_t plan_variant(int v, int n_kv_heads, int rows, int n_sm, AttnPlan* pl
 
 // dtype: VC_DTYPE_BF16 / F32 / F16 (0 / 1 / 3); wide: 16-byte chunks everywhere.
 int variant_for(const AttnArgs& a, int dtype, bool wide) {
-  if (dtype != 1 && wide) {
-    const int size = a.head_dim <= 64 ? 0 : a.head_dim <= 128 ? 1 : 2;
-    const int first = dtype == 0 ? 0 : 10;
-    if (a.rows <= 8) return first + size;
-    if (a.rows <= 16 || size == 2) return first + 3 + size;
-    // 32 or 48 rows a unit: whichever reads the keys in fewer units, then the smaller
-    return first + ((a.rows + 31) / 32 <= (a.rows + 47) / 48 ? 6 : 8) + size;
-  }
-  return (dtype == 1 ? (wide ? 20 : 22) : dtype == 0 ? 24 : 26) + (a.head_dim <= 128 ? 0 : 1);
+  const int size = a.head_dim <= 64 ? 0 : a.head_dim <= 128 ? 1 : 2;
+  if (!wide) return (dtype == 1 ? 25 : dtype == 0 ? 27 : 29) + (size == 2 ? 1 : 0);
+  if (dtype == 1) return a.rows > 4 && size < 2 ? 23 + size : 20 + size;
+  const int first = dtype == 0 ? 0 : 10;
+  if (a.rows <= 8) return first + size;
+  if (a.rows <= 16 || size == 2) return first + 3 + size;
+  // 32 or 48 rows a unit: whichever reads the keys in fewer units, then the smaller
+  return first + ((a.rows + 31) / 32 <= (a.rows + 47) / 48 ? 6 : 8) + size;
 }
 
 }  // namespace
