@@ -1151,13 +1151,19 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_f32_ke
     const int seq = now.seq, len = now.len;
     const int t0 = int(cur - now.base);
     const int t1 = now.nt - t0 < end - cur ? now.nt : t0 + int(end - cur);
-    for (int i = threadIdx.x; i < R * DP; i += kThreads) {
-      const int r = i / DP, d = i - r * DP;
-      qs[r][d] = row0 + r < a.rows && d < a.head_dim ? static_cast<const float*>(a.q)[row_at(a, seq, kvh, row0 + r).q + d] : 0.f;
+    for (int i = threadIdx.x; i < R * kCols; i += kThreads) {
+      const int r = i / kCols, d = (i - r * kCols) * 4;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row0 + r < a.rows && d < a.head_dim)
+        x = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + row_at(a, seq, kvh, row0 + r).q + d);
+      *reinterpret_cast<float4*>(&qs[r][d]) = x;
     }
+    const int group = a.n_heads / a.n_kv_heads;
+    int tok = row0 / group, in_group = row0 - tok * group;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      lim[r] = row0 + r < a.rows ? len - a.n_new + 1 + row_at(a, seq, kvh, row0 + r).tok : 0;
+      lim[r] = row0 + r < a.rows ? len - a.n_new + 1 + tok : 0;
+      if (++in_group == group) in_group = 0, ++tok;
       m[r] = ninf();
       l[r] = 0.f;
 #pragma unroll
