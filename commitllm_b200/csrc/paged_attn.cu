@@ -1311,43 +1311,47 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __g
   constexpr int64_t kPart = part_floats<R, DP>();
   const int unit = row / R * a.n_kv_heads + kvh;
   auto part = [&](int64_t w) { return a.parts + ((w * units + unit) * 2 + (w == wa ? 1 : 0)) * kPart; };
-  float top = ninf();
-  for (int64_t w = wa + threadIdx.x; w <= wb; w += kJoinThreads) top = fmaxf(top, __ldcg(part(w) + R * DP + 2 * r));
-#pragma unroll
-  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-  if (lane == 0) ml_all[warp].x = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(ml_all[0].x, ml_all[1].x), fmaxf(ml_all[2].x, ml_all[3].x));
-  const float ref = top == ninf() ? 0.f : top;
+  // each warp takes every fourth part, relative to the largest maximum it has met
   constexpr int kQ = DP / 4 / 32 ? DP / 4 / 32 : 1;      // float4 a lane
   float4 o[kQ] = {};
-  float l = 0.f;
+  float m = ninf(), l = 0.f;
 #pragma unroll 4
   for (int64_t w = wa + warp; w <= wb; w += kWarps) {
     const float* src = part(w);
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + R * DP + 2 * r));
-    const float f = ex2(ml.x - ref);
-    l += f * ml.y;
+    const float top = fmaxf(m, ml.x), ref = top == ninf() ? 0.f : top;
+    const float g = ex2(m - ref), f = ex2(ml.x - ref);
+    m = top;
+    l = l * g + f * ml.y;
 #pragma unroll
     for (int i = 0; i < kQ; ++i) {
       const int d = (i * 32 + lane) * 4;
       if (d < DP) {
         const float4 x = __ldcg(reinterpret_cast<const float4*>(src + r * DP + d));
-        o[i].x += f * x.x, o[i].y += f * x.y, o[i].z += f * x.z, o[i].w += f * x.w;
+        o[i].x = o[i].x * g + f * x.x, o[i].y = o[i].y * g + f * x.y;
+        o[i].z = o[i].z * g + f * x.z, o[i].w = o[i].w * g + f * x.w;
       }
     }
   }
-  if (lane == 0) ml_all[warp].y = l;
+  if (lane == 0) ml_all[warp] = make_float2(m, l);
 #pragma unroll
   for (int i = 0; i < kQ; ++i) {
     const int d = (i * 32 + lane) * 4;
     if (d < DP) *reinterpret_cast<float4*>(&acc[warp][d]) = o[i];
   }
   __syncthreads();
-  l = ml_all[0].y + ml_all[1].y + ml_all[2].y + ml_all[3].y;
+  const float top = fmaxf(fmaxf(ml_all[0].x, ml_all[1].x), fmaxf(ml_all[2].x, ml_all[3].x));
+  const float ref = top == ninf() ? 0.f : top;
+  float f[kWarps];
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    f[w] = ex2(ml_all[w].x - ref);
+    l += f[w] * ml_all[w].y;
+  }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   for (int d = threadIdx.x; d < a.head_dim; d += kJoinThreads)
-    out[d] = from_f32<T>((acc[0][d] + acc[1][d] + acc[2][d] + acc[3][d]) * inv);
+    out[d] = from_f32<T>((f[0] * acc[0][d] + f[1] * acc[1][d] + f[2] * acc[2][d] + f[3] * acc[3][d]) * inv);
   if (threadIdx.x == 0 && a.lse) a.lse[at.out] = l == 0.f ? ninf() : (top + log2f(l)) * 0.6931471805599453f;
 }
 
