@@ -199,6 +199,8 @@ def rope_frequencies(cfg: RopeConfig, rotary_dim: int, beta_fast: float = 32.0, 
     if cfg.scaling == "linear":
         inv = [f / cfg.factor for f in inv]
     elif cfg.scaling == "llama3":
+        if not 0 < cfg.low_freq_factor < cfg.high_freq_factor:
+            raise ValueError("llama3 scaling needs 0 < low_freq_factor < high_freq_factor")
         out = []
         for f in inv:
             wave = 2.0 * math.pi / f
@@ -210,6 +212,9 @@ def rope_frequencies(cfg: RopeConfig, rotary_dim: int, beta_fast: float = 32.0, 
             out.append(f)
         inv = out
     elif cfg.scaling == "yarn":
+        if not (cfg.theta > 1 and length > 0 and 0 < beta_slow < beta_fast):
+            raise ValueError("yarn scaling needs theta > 1, a positive original length and 0 < beta_slow < beta_fast")
+
         def index(turns):      # the pair that turns this often in the original length
             return r * math.log(length / (turns * 2.0 * math.pi)) / (2.0 * math.log(cfg.theta))
         lo = max(math.floor(index(beta_fast)), 0)
@@ -300,8 +305,10 @@ def paged_attention(cache: PagedCache, layer: int, q: torch.Tensor, seq_lens: to
     q: ``[n_seqs, n_new, n_heads, head_dim]`` in the cache's dtype, any strides
     outside a head (``n_heads`` a multiple of the cache's KV heads; sequence s is
     row s of the block table); seq_lens: int32 ``[n_seqs]`` on the device, the
-    cached rows of each sequence with the new tokens' own.  New token j sees rows
-    ``p < seq_lens[s] - n_new + 1 + j``; a token that sees none gets zeros.
+    cached rows of each sequence with the new tokens' own (0 or less: a padding row of
+    the batch; more than the block table holds: raised by the next ``ctx.sync()``).
+    New token j sees rows ``p < seq_lens[s] - n_new + 1 + j``; a token that sees none
+    gets zeros, and what a token does not see cannot reach its output.
     ``scale`` defaults to ``head_dim ** -0.5``.  Returns ``out`` (shaped as q),
     or ``(out, lse)`` with the float32 natural log of each softmax's sum
     ``[n_seqs, n_new, n_heads]`` (-inf where nothing is seen), from which shards of

@@ -397,8 +397,8 @@ VC_API vc_status vc_kv_transcript_commit(vc_ctx* ctx, const vc_kvt_desc* desc, i
  * v, q_out) share the cache's element type, are contiguous within a head, and
  * have any strides (in elements) between heads and tokens.  These calls
  * allocate nothing, copy nothing from the host and never synchronise: they can
- * be captured.  A page id, position or sequence that leaves the table or the
- * cache is reported by the next vc_ctx_sync as VC_ERANGE; that row is not
+ * be captured.  A page id, position, length or sequence that leaves the table or
+ * the cache is reported by the next vc_ctx_sync as VC_ERANGE; such a row is not
  * touched.
  */
 
@@ -424,7 +424,7 @@ VC_API vc_status vc_rope_append(vc_ctx* ctx, const vc_kv_desc* cache, int32_t la
 /*
  * Attention of the n_new newest tokens of each of the first n_seqs sequences.
  * With n = seq_lens_dev[s] cached rows, the new tokens' own among them, token j
- * sees rows p < n - n_new + 1 + j:
+ * (n <= 0: a padding row of the batch) sees rows p < n - n_new + 1 + j:
  *   out[s][j][h] = sum_p softmax_p(scale * q[s][j][h] . k_p) v_p
  * over the rows of KV head h / (n_heads / n_kv_heads); lse_dev[s][j][h] (NULL:
  * not wanted) = log sum_p exp(scale * q . k_p).  A token that sees no row gets

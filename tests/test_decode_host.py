@@ -39,7 +39,9 @@ def test_yarn_frequencies():
 
 
 @pytest.mark.parametrize("cfg,dim", [(C.RopeConfig(scaling="other"), 64), (C.RopeConfig(), 7), (C.RopeConfig(), 0),
-                                     (C.RopeConfig(theta=0.0), 64), (C.RopeConfig(scaling="linear", factor=0.0), 64)])
+                                     (C.RopeConfig(theta=0.0), 64), (C.RopeConfig(scaling="linear", factor=0.0), 64),
+                                     (C.RopeConfig(theta=1.0, scaling="yarn"), 64),
+                                     (C.RopeConfig(scaling="llama3", low_freq_factor=4.0), 64)])
 def test_frequency_refusals(cfg, dim):
     with pytest.raises(ValueError):
         D.rope_frequencies(cfg, dim)

@@ -168,17 +168,18 @@ def test_attention_unaligned_and_strided(ctx, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
-def test_attention_ignores_what_is_masked(ctx, dtype):
+@pytest.mark.parametrize("heads,dim", [(12, 128), (4, 128), (8, 64), (4, 256), (12, 64), (2, 66)])
+def test_attention_ignores_what_is_masked(ctx, dtype, heads, dim):
     """NaN and infinities in unused slots, past the length, and in rows that only later drafts see."""
     dt = DT[dtype]
     lens = [70, 16, 130]
     new = 4
-    cache, g = make_cache(ctx, 10, lens, 2, 128, 16, dt)
+    cache, g = make_cache(ctx, 10, lens, 2, dim, 16, dt)
     for s, n in enumerate(lens):      # slots past the length
         last = int(cache.block_tables[s, (n - 1) // 16])
         for t, x in ((cache.k_layers[0], math.inf), (cache.v_layers[0], math.nan)):
             t[last, (n - 1) % 16 + 1:] = x
-    q = queries(g, 3, new, 12, 128, dt)
+    q = queries(g, 3, new, heads, dim, dt)
     check_attention(ctx, cache, q, lens)
     n = torch.tensor(lens, dtype=torch.int32, device="cuda")
     for s, ln in enumerate(lens):     # the last two drafts' own rows
@@ -253,6 +254,47 @@ def test_attention_bad_pages_are_reported(ctx):
     out = D.paged_attention(cache, 0, q, n)
     ctx.sync(60000)
     assert torch.equal(out, good)
+
+
+def test_attention_lengths_past_the_table_are_reported(ctx):
+    cache, g = make_cache(ctx, 16, [48, 48], 2, 64, 16, torch.bfloat16)
+    q = queries(g, 2, 1, 4, 64, torch.bfloat16)
+    want = D.paged_attention(cache, 0, q, torch.tensor([48, 30], dtype=torch.int32, device="cuda"))
+    ctx.sync(60000)
+    out = D.paged_attention(cache, 0, q, torch.tensor([49, 30], dtype=torch.int32, device="cuda"))
+    with pytest.raises(Exception, match="block table"):
+        ctx.sync(60000)
+    assert torch.equal(out, want)
+    # a negative length is an empty sequence
+    out = D.paged_attention(cache, 0, q, torch.tensor([-5, 30], dtype=torch.int32, device="cuda"))
+    ctx.sync(60000)
+    assert bool((out[0] == 0).all()) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rows_past_32_bits(ctx, dtype):
+    """A cache of more than 2^32 elements, used at its far end and at its start."""
+    dt, dim, kv, page = DT[dtype], 128, 8, 16
+    pages = (1 << 32) // (page * kv * dim) + 40
+    k, v = (torch.empty(pages, page, kv, dim, dtype=dt, device="cuda") for _ in range(2))
+    table = torch.tensor([[pages - 1, 3, pages - 30, pages - 2], [7, pages - 3, 0, pages - 4]], dtype=torch.int32,
+                         device="cuda")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(21)
+    for p in table.flatten().tolist():
+        for t in (k, v):
+            t[p] = torch.randn(page, kv, dim, generator=g, device="cuda").to(dt)
+    cache = D.PagedCache(ctx, [k], [v], table)
+    check_attention(ctx, cache, queries(g, 2, 2, 16, dim, dt), [64, 50])
+    x = torch.randn(3, 2, kv, dim, generator=g, device="cuda").to(dt)
+    pos = torch.tensor([5, 63], dtype=torch.int32, device="cuda")
+    D.rope_append(cache, 0, x[0], x[1], x[2], pos, D.rope_table(ctx, C.RopeConfig(), dim),
+                  seq_ids=torch.tensor([0, 1], dtype=torch.int32, device="cuda"))
+    ctx.sync(60000)
+    inv, f = D.rope_frequencies(C.RopeConfig(), dim)
+    want, tol = rope_reference(x[1], pos, inv, f, False)
+    for t, (p, slot) in enumerate(((pages - 1, 5), (pages - 4, 15))):
+        assert close_rows(k[p, slot], want[t], tol[t]) and torch.equal(v[p, slot], x[2, t])
 
 
 def test_attention_graph_replay_grows_with_its_tensors(ctx):

@@ -210,6 +210,26 @@ def test_verify_sequences_with_fewer_drafts(ctx):
         check(ctx, logits, drafts, u, t, probs)
 
 
+@pytest.mark.parametrize("k", [15, 16, 17, 40])
+def test_verify_many_drafts(ctx, k):
+    """Runs of kept drafts past 16 positions, ended at every kind of place."""
+    rng = np.random.default_rng(k)
+    S, V = 12, 600
+    l = rng.standard_normal((S, k + 1, V)).astype(np.float32)
+    best = rng.integers(0, V, (S, k + 1))
+    l[np.arange(S)[:, None], np.arange(k + 1)[None], best] += 25.0
+    drafts = best[:, :k].astype(np.int32)
+    for s, end in enumerate((0, 1, 14, 15, 16, 17, 31, 32, 33, k - 1)):
+        if end < k:
+            drafts[s, end] = (drafts[s, end] + 1) % V
+    t = np.where(np.arange(S) % 3 == 0, 0.0, 1.0).astype(np.float32)
+    u = rng.random((S, k + 1))
+    _, n = check(ctx, torch.tensor(l, device="cuda"), drafts, u, t)
+    assert n[-1] == k + 1 and n[3] == min(16, k + 1)
+    probs = torch.softmax(torch.tensor(l[:, :k], device="cuda") + 1, -1)
+    check(ctx, torch.tensor(l, device="cuda"), drafts, u, t, probs)
+
+
 def test_verify_draft_distribution_equal_to_the_targets(ctx):
     """Nothing of p lies above q: a refused draft's replacement comes from p itself."""
     V = 64
