@@ -133,17 +133,18 @@ __device__ Place locate(const AttnArgs& a, int range) {
 }
 
 // The sequence that holds a tile, and what a warp needs of it.
+// Tiles are counted from the range's first one (the 32-bit registers are needed).
 struct Cursor {
   int seq, len, nt;
-  int64_t base;       // its first tile of keys
-  __device__ __forceinline__ void at(const AttnArgs& a, int s, int64_t b) {
+  int base;           // its first tile of keys
+  __device__ __forceinline__ void at(const AttnArgs& a, int s, int b) {
     seq = s, base = b;
     len = int(seq_len(a, s));
     nt = (len + kTile - 1) / kTile;
     if (nt) base += kStart;
   }
   // The first tile of keys from `tile` on, if it is before `end`; else end.
-  __device__ __forceinline__ int64_t advance(const AttnArgs& a, int64_t tile, int64_t end) {
+  __device__ __forceinline__ int advance(const AttnArgs& a, int tile, int end) {
     while (tile < end && tile >= base + nt) at(a, seq + 1, base + nt);
     if (tile < base) tile = base;
     return tile < end ? tile : end;
@@ -480,28 +481,24 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
   const int group = a.n_heads / a.n_kv_heads;
   const Place pl = locate<kWarps>(a, range);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t chunk = chunk_of(pl.total, a.n_ranges);
-  const int64_t begin = int64_t(range) * chunk;
-  const int64_t end = begin + chunk < pl.total ? begin + chunk : pl.total;
-  if (begin >= end) return;
-  float* parts = a.parts + int64_t(blockIdx.x) * 2 * part_floats<R, DP>();
+  const int64_t chunk = chunk_of(pl.total, a.n_ranges), first = int64_t(range) * chunk;
+  if (first >= pl.total) return;
+  const int end = int(pl.total - first < chunk ? pl.total - first : chunk);
 
   // ---- loading: lane i < 16 finds key i's row, one stage before it is copied
   Cursor ahead;
-  ahead.at(a, pl.seq, pl.seq_base);
-  int64_t next = begin;                // tile the registers below describe
-  int page = 0, slot = 0;
-  bool real = false;
+  ahead.at(a, pl.seq, int(pl.seq_base - first));
+  int next = 0;                // tile the registers below describe
+  int page = 0, slot = -1;             // -1: the lane has no row
   auto look = [&]() {
-    real = false;
+    slot = -1;
     next = ahead.advance(a, next, end);
     if (next < end) {
-      const int p = int(next - ahead.base) * kTile + warp * 16 + lane;
+      const int p = (next - ahead.base) * kTile + warp * 16 + lane;
       if (lane < 16 && p < ahead.len) {
         const int block = unsigned(p) / unsigned(a.block_size);
         page = __ldg(a.block_tables + int64_t(ahead.seq) * a.max_blocks + block);
         slot = p - block * a.block_size;
-        real = true;
       }
     }
   };
@@ -509,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
   auto issue = [&]() {
     if (next < end) {
       int64_t off = -1;
-      if (real) {
+      if (slot >= 0) {
         off = int64_t(page) * a.stride_page + int64_t(slot) * a.stride_row;
         if (page < 0 || off + a.row_span > a.cache_elems) {
           *a.err = 1;
@@ -547,12 +544,12 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
   int lim[NT];
   int use = 0;                         // stage to use
   Cursor now;
-  now.at(a, pl.seq, pl.seq_base);
-  int64_t cur = begin;
+  now.at(a, pl.seq, int(pl.seq_base - first));
+  int cur = 0;
   while ((cur = now.advance(a, cur, end)) < end) {
     const int seq = now.seq, len = now.len;
-    const int t0 = int(cur - now.base);
-    const int t1 = now.nt - t0 < end - cur ? now.nt : t0 + int(end - cur);
+    const int t0 = cur - now.base;
+    const int t1 = now.nt - t0 < end - cur ? now.nt : t0 + (end - cur);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = row0 + h * 8 + n;
@@ -641,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
     // the four warps' results, eight rows at a time; a part that begins its sequence
     // goes to slot 1, one that continues it to slot 0
     const bool whole = t0 == 0 && t1 == now.nt;
-    float* part = parts + (t0 == 0 ? part_floats<R, DP>() : 0);
+    float* part = a.parts + (int64_t(blockIdx.x) * 2 + (t0 == 0 ? 1 : 0)) * part_floats<R, DP>();
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       float sum = l[t] + __shfl_xor_sync(~0u, l[t], 1);
@@ -700,29 +697,25 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
   const int group = a.n_heads / a.n_kv_heads;
   const Place pl = locate<kW>(a, range);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t chunk = chunk_of(pl.total, a.n_ranges);
-  const int64_t begin = int64_t(range) * chunk;
-  const int64_t end = begin + chunk < pl.total ? begin + chunk : pl.total;
-  if (begin >= end) return;
-  float* parts = a.parts + int64_t(blockIdx.x) * 2 * part_floats<R, DP>();
+  const int64_t chunk = chunk_of(pl.total, a.n_ranges), first = int64_t(range) * chunk;
+  if (first >= pl.total) return;
+  const int end = int(pl.total - first < chunk ? pl.total - first : chunk);
 
   // ---- loading: a warp copies every kW-th group of kRowsPerCopy rows; lane i finds the i-th of its rows
   Cursor ahead;
-  ahead.at(a, pl.seq, pl.seq_base);
-  int64_t next = begin;
-  int page = 0, slot = 0;
-  bool real = false;
+  ahead.at(a, pl.seq, int(pl.seq_base - first));
+  int next = 0;
+  int page = 0, slot = -1;             // -1: the lane has no row
   const int my_group = warp + lane / kRowsPerCopy * kW, my_row = my_group * kRowsPerCopy + lane % kRowsPerCopy;
   auto look = [&]() {
-    real = false;
+    slot = -1;
     next = ahead.advance(a, next, end);
     if (next < end) {
-      const int p = int(next - ahead.base) * kTile + my_row;
+      const int p = (next - ahead.base) * kTile + my_row;
       if (lane < kCopies * kRowsPerCopy && my_row < kTile && p < ahead.len) {
         const int block = unsigned(p) / unsigned(a.block_size);
         page = __ldg(a.block_tables + int64_t(ahead.seq) * a.max_blocks + block);
         slot = p - block * a.block_size;
-        real = true;
       }
     }
   };
@@ -730,7 +723,7 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
   auto issue = [&]() {
     if (next < end) {
       int64_t off = -1;
-      if (real) {
+      if (slot >= 0) {
         off = int64_t(page) * a.stride_page + int64_t(slot) * a.stride_row;
         if (page < 0 || off + a.row_span > a.cache_elems) {
           *a.err = 1;
@@ -768,12 +761,12 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
   int lim[2];
   int use = 0;
   Cursor now;
-  now.at(a, pl.seq, pl.seq_base);
-  int64_t cur = begin;
+  now.at(a, pl.seq, int(pl.seq_base - first));
+  int cur = 0;
   while ((cur = now.advance(a, cur, end)) < end) {
     const int seq = now.seq, len = now.len;
-    const int t0 = int(cur - now.base);
-    const int t1 = now.nt - t0 < end - cur ? now.nt : t0 + int(end - cur);
+    const int t0 = cur - now.base;
+    const int t1 = now.nt - t0 < end - cur ? now.nt : t0 + (end - cur);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = wrow0 + h * 8 + n;
@@ -867,7 +860,7 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
     // the key halves' results: query rows 0-7 or 8-15 of each row tile, and half of their
     // elements, at a time; buffer row 8 * wr + n is query row row0 + 16 * wr + 8 * h + n
     const bool whole = t0 == 0 && t1 == now.nt;
-    float* part = parts + (t0 == 0 ? part_floats<R, DP>() : 0);
+    float* part = a.parts + (int64_t(blockIdx.x) * 2 + (t0 == 0 ? 1 : 0)) * part_floats<R, DP>();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float sum = l[h] + __shfl_xor_sync(~0u, l[h], 1);
@@ -1032,23 +1025,22 @@ __global__ void __launch_bounds__(kThreads) paged_attn_fma_kernel(const __grid_c
   const int rt = unit / a.n_kv_heads, kvh = unit - rt * a.n_kv_heads, row0 = rt * R;
   const Place pl = locate<kWarps>(a, range);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t chunk = chunk_of(pl.total, a.n_ranges);
-  int64_t cur = int64_t(range) * chunk;
-  const int64_t end = cur + chunk < pl.total ? cur + chunk : pl.total;
+  const int64_t chunk = chunk_of(pl.total, a.n_ranges), first = int64_t(range) * chunk;
+  if (first >= pl.total) return;
+  const int end = int(pl.total - first < chunk ? pl.total - first : chunk);
+  int cur = 0;
   Cursor now;
-  now.at(a, pl.seq, pl.seq_base);
-  float* parts = a.parts + int64_t(blockIdx.x) * 2 * part_floats<R, DP>();
-  if (cur >= end) return;
+  now.at(a, pl.seq, int(pl.seq_base - first));
   while ((cur = now.advance(a, cur, end)) < end) {
     const int seq = now.seq, len = now.len, nt = now.nt;
-    const int t0 = int(cur - now.base);
-    const int t1 = nt - t0 < end - cur ? nt : t0 + int(end - cur);
+    const int t0 = cur - now.base;
+    const int t1 = nt - t0 < end - cur ? nt : t0 + (end - cur);
     Core core;
     core.run(a, seq, kvh, row0, len, t0, t1, mg.o[0]);      // the queries sit where the outputs will
     __syncthreads();
     core.store(mg);
     // a part that begins its sequence goes to slot 1, one that continues it to slot 0
-    float* part = parts + (t0 == 0 ? part_floats<R, DP>() : 0);
+    float* part = a.parts + (int64_t(blockIdx.x) * 2 + (t0 == 0 ? 1 : 0)) * part_floats<R, DP>();
     emit<T, kWarps, R, DP, DP>(a, mg, {seq, kvh, row0, t0 == 0 && t1 == nt ? nullptr : part, part + R * DP}, 8, true, 0);
     cur += t1 - t0;
   }
@@ -1088,30 +1080,26 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_f32_ke
   const int rt = unit / a.n_kv_heads, kvh = unit - rt * a.n_kv_heads, row0 = rt * R;
   const Place pl = locate<kWarps>(a, range);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t chunk = chunk_of(pl.total, a.n_ranges);
-  const int64_t begin = int64_t(range) * chunk;
-  const int64_t end = begin + chunk < pl.total ? begin + chunk : pl.total;
-  if (begin >= end) return;
-  float* parts = a.parts + int64_t(blockIdx.x) * 2 * part_floats<R, DP>();
+  const int64_t chunk = chunk_of(pl.total, a.n_ranges), first = int64_t(range) * chunk;
+  if (first >= pl.total) return;
+  const int end = int(pl.total - first < chunk ? pl.total - first : chunk);
 
   // ---- loading: lane i < 8 finds key i's row, one stage before it is copied
   Cursor ahead;
-  ahead.at(a, pl.seq, pl.seq_base);
-  int64_t next = begin;                // tile, and which 8 of the warp's 16 keys of it
+  ahead.at(a, pl.seq, int(pl.seq_base - first));
+  int next = 0;                // tile, and which 8 of the warp's 16 keys of it
   int next_half = 0;
-  int page = 0, slot = 0;
-  bool real = false;
+  int page = 0, slot = -1;             // -1: the lane has no row
   auto look = [&]() {
-    real = false;
-    const int64_t t = ahead.advance(a, next, end);
+    slot = -1;
+    const int t = ahead.advance(a, next, end);
     if (t != next) next = t, next_half = 0;
     if (next < end) {
-      const int p = int(next - ahead.base) * kTile + warp * 16 + next_half * 8 + lane;
+      const int p = (next - ahead.base) * kTile + warp * 16 + next_half * 8 + lane;
       if (lane < 8 && p < ahead.len) {
         const int block = unsigned(p) / unsigned(a.block_size);
         page = __ldg(a.block_tables + int64_t(ahead.seq) * a.max_blocks + block);
         slot = p - block * a.block_size;
-        real = true;
       }
     }
   };
@@ -1119,7 +1107,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_f32_ke
   auto issue = [&]() {
     if (next < end) {
       int64_t off = -1;
-      if (real) {
+      if (slot >= 0) {
         off = int64_t(page) * a.stride_page + int64_t(slot) * a.stride_row;
         if (page < 0 || off + a.row_span > a.cache_elems) {
           *a.err = 1;
@@ -1154,12 +1142,12 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_f32_ke
   int lim[R];
   int use = 0;
   Cursor now;
-  now.at(a, pl.seq, pl.seq_base);
-  int64_t cur = begin;
+  now.at(a, pl.seq, int(pl.seq_base - first));
+  int cur = 0;
   while ((cur = now.advance(a, cur, end)) < end) {
     const int seq = now.seq, len = now.len;
-    const int t0 = int(cur - now.base);
-    const int t1 = now.nt - t0 < end - cur ? now.nt : t0 + int(end - cur);
+    const int t0 = cur - now.base;
+    const int t1 = now.nt - t0 < end - cur ? now.nt : t0 + (end - cur);
     for (int i = threadIdx.x; i < R * kCols; i += kThreads) {
       const int r = i / kCols, d = (i - r * kCols) * 4;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1265,7 +1253,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_f32_ke
         if (lane < 8) *reinterpret_cast<float4*>(&mg.o[warp][r][(i * 8 + g) * 4]) = make_float4(y[0], y[1], y[2], y[3]);
       }
     }
-    float* part = parts + (t0 == 0 ? part_floats<R, DP>() : 0);
+    float* part = a.parts + (int64_t(blockIdx.x) * 2 + (t0 == 0 ? 1 : 0)) * part_floats<R, DP>();
     emit<float, kWarps, R, DP, DP>(a, mg, {seq, kvh, row0, t0 == 0 && t1 == now.nt ? nullptr : part, part + R * DP}, 8, true, 0);
     cur += t1 - t0;
   }
