@@ -60,11 +60,12 @@ def _handle(ctx: Context) -> int:
     return ctx._h.value or ctx.handle.value
 
 
-def _empty(ctx: Context, shape, dtype) -> torch.Tensor:
-    # Context.empty without the stream switch when the stream is current already
+def _empty(ctx: Context, like: torch.Tensor, shape, dtype=None) -> torch.Tensor:
+    # Context.empty without the stream switch when the stream is current already;
+    # new_empty costs two thirds of torch.empty
     if torch._C._cuda_getCurrentRawStream(ctx.device) == ctx.stream.cuda_stream:
-        return torch.empty(shape, dtype=dtype, device=ctx.stream.device)
-    return ctx.empty(shape, dtype=dtype)
+        return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
+    return ctx.empty(shape, dtype=dtype or like.dtype)
 
 
 def _empty_like(ctx: Context, t: torch.Tensor) -> torch.Tensor:
@@ -338,10 +339,10 @@ def paged_attention(cache: PagedCache, layer: int, q: torch.Tensor, seq_lens: to
         _on(ctx, out, "out")
         if out.dtype != cache.dtype or out.shape != q.shape or not out.is_contiguous():
             raise ValueError("out must be contiguous, of q's shape and dtype")
-    lse = _empty(ctx, (S, N, H), torch.float32) if return_lse else None
+    lse = _empty(ctx, q, (S, N, H), torch.float32) if return_lse else None
     need = cache._workspace.get((N, H)) or cache.workspace_bytes(N, H)
     if workspace is None:
-        workspace = _empty(ctx, need, torch.uint8)
+        workspace = _empty(ctx, seq_lens, need // 4)        # (a multiple of 16 bytes)
     else:
         _on(ctx, workspace, "workspace")
         if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
@@ -405,13 +406,13 @@ def verify_tokens(ctx: Context, logits: torch.Tensor, drafts: torch.Tensor, unif
                 and draft_probs.get_device() == dev):
             raise ValueError(f"draft_probs must be float32 [{S}, {N - 1}, {V}] on device {dev}, contiguous within a row")
         probs = draft_probs.data_ptr()
-    tokens = _empty(ctx, (S, N), torch.int32)
-    counts = _empty(ctx, (S,), torch.int32)
+    tokens = _empty(ctx, drafts, (S, N))
+    counts = _empty(ctx, drafts, (S,))
     if S == 0:
         return tokens, counts
     if workspace is None:
         need = S * N * _VERIFY_ROW_BYTES
-        workspace = _empty(ctx, need, torch.uint8)
+        workspace = _empty(ctx, drafts, need // 4)
     else:
         _on(ctx, workspace, "workspace")
         if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
