@@ -9,10 +9,9 @@
 //
 // Work split.  All sequences' keys, in tiles of 64 (and what starting a sequence costs,
 // counted as tiles), are laid end to end and cut into equal contiguous ranges; a worker
-// CTA takes one range for one unit (KV
-// head, tile of up to R query rows).  The number of ranges is set so that the
-// workers are all resident at once, so a ragged batch and a single long sequence
-// both spread evenly without the host knowing the lengths.  The units of a range
+// CTA takes one range for one unit (KV head, tile of up to R query rows).  The number
+// of ranges is set so that the workers are all resident at once, so a ragged batch and
+// a single long sequence both spread evenly without the host knowing the lengths.  The units of a range
 // are neighbouring CTAs: they read the heads of the same cache rows, which lie
 // side by side in memory, at about the same time.  A sequence that lies in one
 // range is written by its worker; the others' parts (running maximum, sum and
@@ -52,8 +51,8 @@ __device__ __forceinline__ int64_t key_tiles(const AttnArgs& a, int s) {
 }
 
 // What a sequence counts for when the ranges are cut: kStart tiles for starting it
-// (queries to read, a result to write: about two tiles' time) and its keys' tiles
-// behind them.
+// (queries to read, a result to write: about two tiles' time; counting it took 1024-token
+// drafts from 31 to 27 us) and its keys' tiles behind them.
 constexpr int kStart = 2;
 __device__ __forceinline__ int64_t seq_tiles(const AttnArgs& a, int s) {
   const int64_t n = key_tiles(a, s);
@@ -660,10 +659,10 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
 // held all rows would need 255 registers and leave two warps a scheduler; here it is
 // three, with 92 B/clk of shared memory reads at the HBM's rate, of 128.  Bound by
 // instruction latency, not by the bytes: 35 rows over 16 sequences of up to 8192 (159
-// MB) take 70 us, eight times longer ones 334 us where the bytes take 195; tensor pipe
-// 38 %, 0.37 instructions a cycle and scheduler, most stalls on fixed latencies.  Two
-// blocks of 16 keys side by side gave 8 % over one, a maximum that lanes test alone
-// nothing here.
+// MB) take 68 us, eight times longer ones 323 us where the bytes take 195 (21 rows: 234);
+// tensor pipe 38 %, 0.37 instructions a cycle and scheduler, most stalls on fixed
+// latencies.  Two blocks of 16 keys side by side gave 8 % over one.  Row tiles of 8, five
+// warps a scheduler with 96 registers, spilled and took 91 us.
 template <int WR, int DP>
 struct RowsShape {
   static constexpr int kWarpsHere = WR * 2;
@@ -1047,11 +1046,12 @@ __global__ void __launch_bounds__(kThreads) paged_attn_fma_kernel(const __grid_c
 }
 
 // f32 rows on 16-byte boundaries: the ring of paged_attn_tc_kernel in stages of 8 keys,
-// with the products in f32 FMAs (512 a lane for 8 keys and 8 query rows, under half of
-// what a SM does while it loads those keys).  Eight lanes share a key, four keys at a
-// time; a lane's elements of a row are chunks i * 8 + lane % 8 of four.  The first
-// version loaded straight into registers, one step ahead: 4.0 TB/s, 26 us for a call of
-// 20 MB that spends most of its time on the way from load to load.
+// with the products in f32 FMAs (512 a lane for 8 keys and 8 query rows).  Eight lanes
+// share a key, four keys at a time; a lane's elements of a row are chunks i * 8 + lane %
+// 8 of four.  Measured on 318 MB: 4 query rows 62 us (5.2 TB/s; 79 with loads straight
+// into registers, one step ahead), 7 rows 82 us, where the instructions bound it; a call
+// of 20 MB and 6 rows takes 20.6 us, most of it starting up.  Packed pairs of FMAs
+// measured no faster.
 template <int R, int DP>
 struct F32Shape {
   static constexpr int kKeys = 8;

@@ -15,6 +15,11 @@
 // partner of the second half (neighbouring pairs: one chunk), or one chunk of
 // the unrotated rest; narrower chunks where alignment or an odd rotary_dim asks
 // for them.
+//
+// Measured: 8192 tokens of 64 + 8 + 8 heads of 128 in bf16 (336 MB moved) 57.7 us, 5.8
+// TB/s; 256 tokens 6.3 us, one token 4.3 us (the launch, then positions, angles and rows
+// one behind the other).  128 threads a CTA gave 3 % over 256; loading four units a
+// thread ahead of the angles halved the CTAs an SM holds and took 181 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

