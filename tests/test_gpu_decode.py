@@ -453,6 +453,66 @@ def test_rope_append_many_tokens_and_default_sequences(ctx):
     assert torch.equal(kv[1][table[:, 0].long(), pos.long()], x[2])
 
 
+def test_rope_append_is_captured_and_replayed(ctx):
+    """A captured step replayed with other tokens, positions and pages."""
+    stream = torch.cuda.Stream()
+    c2 = C.Context(0, stream)
+    cache, g = make_cache(c2, 22, [64, 64], 2, 64, 16, torch.bfloat16, fill=0.0)
+    x = torch.zeros(3, 2, 2, 64, dtype=torch.bfloat16, device="cuda")
+    pos = torch.zeros(2, dtype=torch.int32, device="cuda")
+    rope = D.rope_table(c2, CONFIGS["yarn"], 64)
+    inv, f = D.rope_frequencies(CONFIGS["yarn"], 64)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        D.rope_append(cache, 0, x[0], x[1], x[2], pos, rope)
+        stream.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=stream):
+            out = D.rope_append(cache, 0, x[0], x[1], x[2], pos, rope)
+    for p in ([3, 40], [63, 0]):
+        x.copy_(torch.randn(3, 2, 2, 64, generator=g, device="cuda"))
+        pos.copy_(torch.tensor(p, dtype=torch.int32))
+        cache.block_tables.copy_(cache.block_tables.flip(0))
+        torch.cuda.synchronize()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert close_rows(out, *rope_reference(x[0], pos, inv, f, False))
+        wk, tk = rope_reference(x[1], pos, inv, f, False)
+        for s in range(2):
+            page, slot = int(cache.block_tables[s, p[s] // 16]), p[s] % 16
+            assert close_rows(cache.k_layers[0][page, slot], wk[s], tk[s])
+            assert torch.equal(cache.v_layers[0][page, slot], x[2, s])
+    del gr
+    c2.close()
+
+
+def test_contexts_on_two_streams_at_once(ctx):
+    """Two contexts on their own streams, neither the current one, working at the same time: the results of one
+    after the other."""
+    lens = [3000, 170, 0, 1024]
+    ctxs = [C.Context(0, torch.cuda.Stream()) for _ in range(2)]
+    made = [make_cache(c, 40 + i, lens, 2, 128, 16, torch.bfloat16) for i, c in enumerate(ctxs)]
+    qs = [queries(g, 4, 2, 8, 128, torch.bfloat16) for _, g in made]
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    want = []
+    for (cache, _), q in zip(made, qs):
+        want.append(D.paged_attention(cache, 0, q, n, return_lse=True))
+        cache.ctx.sync(60000)
+    got = [[], []]
+    for _ in range(10):
+        for i, ((cache, _), q) in enumerate(zip(made, qs)):
+            got[i].append(D.paged_attention(cache, 0, q, n, return_lse=True))
+    for c in ctxs:
+        c.sync(60000)
+    for i in range(2):
+        for out, lse in got[i]:
+            assert torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])
+        check_attention(ctxs[i], made[i][0], qs[i], lens)
+    for c in ctxs:
+        c.close()
+
+
 def test_rope_append_reports_rows_outside_the_cache(ctx):
     cache, g = make_cache(ctx, 20, [32, 32], 1, 64, 16, torch.bfloat16, fill=0.0)
     x = torch.randn(3, 1, 64, generator=g, device="cuda").to(torch.bfloat16)
