@@ -670,7 +670,11 @@ struct RowsShape {
   static constexpr int kStages = DP == 64 ? 6 : 3;
   static constexpr int kRing = kStages * kStage;             // 96 KB
   using Mg = Merge<2, WR * 8, DP / 2>;      // 8 rows of each row tile, half of their elements
-  static constexpr size_t kSmem = kRing + sizeof(Mg);
+  // three row tiles leave 168 registers a thread: their queries stay in shared memory,
+  // where the outputs will be
+  static constexpr bool kQShared = WR > 2;
+  static constexpr size_t kTail = kQShared && WR * 16 * DP * 2 > sizeof(Mg) ? WR * 16 * DP * 2 : sizeof(Mg);
+  static constexpr size_t kSmem = kRing + kTail;
 };
 
 template <typename T, int WR, int DP>
@@ -754,7 +758,9 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
   for (int i = 0; i < kStages - 1; ++i) issue();
 
   const int key = ((lane >> 4) << 3) + (lane & 7), half = (lane >> 3) & 1, flip = lane & 7;
-  uint32_t q[KS][4];
+  uint32_t q[Shape::kQShared ? 1 : KS][4];
+  const int qrow = wr * 16 + half * 8 + (lane & 7);
+  const uint32_t qs = smem_addr(smem + Shape::kRing) + qrow * (DP * 2);
   float o[2][KS][4];
   float m[2], l[2];
   int lim[2];
@@ -766,18 +772,31 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
     const int seq = now.seq, len = now.len;
     const int t0 = cur - now.base;
     const int t1 = now.nt - t0 < end - cur ? now.nt : t0 + (end - cur);
+    if constexpr (Shape::kQShared) {
+      for (int i = threadIdx.x; i < R * kCols; i += WR * 64) {
+        const int r = i / kCols, col = i - r * kCols;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (row0 + r < a.rows && col * 8 < a.head_dim)
+          x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + row_at(a, seq, kvh, row0 + r).q + col * 8);
+        x.x ^= a.q_sign, x.y ^= a.q_sign, x.z ^= a.q_sign, x.w ^= a.q_sign;
+        *reinterpret_cast<uint4*>(smem + Shape::kRing + r * (DP * 2) + ((col ^ (r & 7)) << 4)) = x;
+      }
+      __syncthreads();
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = wrow0 + h * 8 + n;
       const bool has = r < a.rows;
-      const T* src = static_cast<const T*>(a.q) + row_at(a, seq, kvh, has ? r : 0).q;
+      if constexpr (!Shape::kQShared) {
+        const T* src = static_cast<const T*>(a.q) + row_at(a, seq, kvh, has ? r : 0).q;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int e = ks * 16 + x * 8 + 2 * c;
-          q[ks][h + 2 * x] = has && e < a.head_dim ? *reinterpret_cast<const uint32_t*>(src + e) ^ a.q_sign : 0u;
-        }
+          for (int x = 0; x < 2; ++x) {
+            const int e = ks * 16 + x * 8 + 2 * c;
+            q[ks][h + 2 * x] = has && e < a.head_dim ? *reinterpret_cast<const uint32_t*>(src + e) ^ a.q_sign : 0u;
+          }
+      }
       lim[h] = has ? len - a.n_new + 1 + r / group : 0;
       m[h] = ninf();
       l[h] = 0.f;
@@ -801,12 +820,20 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
       float s[2][2][4] = {};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
+        uint32_t f[4];
+        if constexpr (Shape::kQShared) {
+          // blocks of a Q fragment: rows 0-7 and 8-15 of the left half, then of the right
+          ldsm(qs + (((ks * 2 + (lane >> 4)) ^ flip) << 4), f);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f[j] = q[ks][j];
+        }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           uint32_t k[4];
           ldsm(krow + b * kBlock + (((ks * 2 + half) ^ flip) << 4), k);
-          B::mma(s[b][0], q[ks][0], q[ks][1], q[ks][2], q[ks][3], k[0], k[1]);
-          B::mma(s[b][1], q[ks][0], q[ks][1], q[ks][2], q[ks][3], k[2], k[3]);
+          B::mma(s[b][0], f[0], f[1], f[2], f[3], k[0], k[1]);
+          B::mma(s[b][1], f[0], f[1], f[2], f[3], k[2], k[3]);
         }
       }
       const bool all_seen = p0 + 32 <= sure;
@@ -859,6 +886,7 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
     // the key halves' results: query rows 0-7 or 8-15 of each row tile, and half of their
     // elements, at a time; buffer row 8 * wr + n is query row row0 + 16 * wr + 8 * h + n
     const bool whole = t0 == 0 && t1 == now.nt;
+    if constexpr (Shape::kQShared) __syncthreads();      // the queries make place
     float* part = a.parts + (int64_t(blockIdx.x) * 2 + (t0 == 0 ? 1 : 0)) * part_floats<R, DP>();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
