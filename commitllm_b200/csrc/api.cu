@@ -1107,6 +1107,8 @@ vc_status check_attn(const vc_kv_desc* d, int32_t layer, int32_t n_new, int32_t 
     return fail(VC_EINVAL, "%s: %d query heads are no multiple of %d KV heads", fn, n_heads, d->n_kv_heads);
   if (int64_t(n_new) * (n_heads / d->n_kv_heads) > 65535)
     return fail(VC_ENOTSUP, "%s: more than 65535 query rows of one KV head", fn);
+  if (int64_t(d->max_blocks_per_seq) * d->block_size > (int64_t(1) << 30))
+    return fail(VC_ENOTSUP, "%s: a block table of more than 2^30 rows a sequence", fn);
   return VC_OK;
 }
 

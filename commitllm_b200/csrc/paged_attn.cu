@@ -913,34 +913,21 @@ __global__ void __launch_bounds__(WR * 64, 2) paged_attn_rows_kernel(const __gri
 // ----------------------------------------------- rows of any alignment: FMAs
 
 // Eight lanes share a key (four keys at a time, 16 per warp and tile); each holds
-// DP / 8 of its elements.  V elements a load; element (i, e) of lane g is
-// (i * 8 + g) * V + e.  The query rows sit in shared memory as f32.
-template <typename T, int V, int DP>
+// DP / 8 of its elements, one a load: number i of lane g is i * 8 + g.  The query rows
+// sit in shared memory as f32.
+template <typename T, int DP>
 struct Fma {
   static constexpr int R = 4;
   static constexpr int kRows = R, kDP = DP;
-  static constexpr int NL = DP / 8 / V;       // loads of a row
-  float o[R][NL * V];
+  static constexpr int NL = DP / 8;           // elements of a lane
+  float o[R][NL];
   float m[R], l[R];
   int lim[R];
 
-  struct alignas(sizeof(T) * V) Chunk {
-    T v[V];
-  };
-
-  __device__ __forceinline__ void load(float (&x)[NL * V], const T* src, bool real, int dim) {
+  __device__ __forceinline__ void load(float (&x)[NL], const T* src, bool real, int dim) {
     const int g = threadIdx.x & 7;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int e = (i * 8 + g) * V;
-#pragma unroll
-      for (int j = 0; j < V; ++j) x[i * V + j] = 0.f;
-      if (real && e < dim) {
-        const Chunk ch = *reinterpret_cast<const Chunk*>(src + e);
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[i * V + j] = to_f32(ch.v[j]);
-      }
-    }
+    for (int i = 0; i < NL; ++i) x[i] = real && i * 8 + g < dim ? to_f32(src[i * 8 + g]) : 0.f;
   }
 
   __device__ __forceinline__ void run(const AttnArgs& a, int seq, int kvh, int row0, int len, int t0, int t1,
@@ -960,13 +947,13 @@ struct Fma {
       m[r] = ninf();
       l[r] = 0.f;
 #pragma unroll
-      for (int i = 0; i < NL * V; ++i) o[r][i] = 0.f;
+      for (int i = 0; i < NL; ++i) o[r][i] = 0.f;
     }
     __syncthreads();
     const T* kb = static_cast<const T*>(a.k) + kvh * a.stride_head;
     const T* vb = static_cast<const T*>(a.v) + kvh * a.stride_head;
     const int n = (t1 - t0) * 4;               // steps of four keys
-    float kx[NL * V], vx[NL * V];
+    float kx[NL], vx[NL];
     int p = t0 * kTile + warp * 16 + (lane >> 3);
     int64_t off = p < len ? row_of(a, seq, p) : -1;
     load(kx, kb + off, off >= 0, a.head_dim);
@@ -983,8 +970,7 @@ struct Fma {
       for (int e = 0; e < NL; ++e)
 #pragma unroll
         for (int r = 0; r < R; ++r)
-#pragma unroll
-          for (int j = 0; j < V; ++j) s[r] = fmaf(qs[r][(e * 8 + g) * V + j], kx[e * V + j], s[r]);
+          s[r] = fmaf(qs[r][e * 8 + g], kx[e], s[r]);
       load(kx, kb + offn, offn >= 0, a.head_dim);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -998,7 +984,7 @@ struct Fma {
           const float f = m[r] == ninf() ? 0.f : ex2(m[r] - top);
           l[r] *= f;
 #pragma unroll
-          for (int j = 0; j < NL * V; ++j) o[r][j] *= f;
+          for (int j = 0; j < NL; ++j) o[r][j] *= f;
           m[r] = top;
         }
         const float ref = m[r] == ninf() ? 0.f : m[r];
@@ -1006,7 +992,7 @@ struct Fma {
         l[r] += e;
         if (seen) {
 #pragma unroll
-          for (int j = 0; j < NL * V; ++j) o[r][j] = fmaf(e, vx[j], o[r][j]);
+          for (int j = 0; j < NL; ++j) o[r][j] = fmaf(e, vx[j], o[r][j]);
         }
       }
       load(vx, vb + offn, offn >= 0, a.head_dim);
@@ -1028,14 +1014,12 @@ struct Fma {
       sum += __shfl_xor_sync(~0u, sum, 16);
       if (lane == 0) mg.m[warp][r] = top, mg.l[warp][r] = sum;
 #pragma unroll
-      for (int i = 0; i < NL; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float x = o[r][i * V + j] * f;
-          x += __shfl_xor_sync(~0u, x, 8);
-          x += __shfl_xor_sync(~0u, x, 16);
-          if (lane < 8) mg.o[warp][r][(i * 8 + g) * V + j] = x;
-        }
+      for (int i = 0; i < NL; ++i) {
+        float x = o[r][i] * f;
+        x += __shfl_xor_sync(~0u, x, 8);
+        x += __shfl_xor_sync(~0u, x, 16);
+        if (lane < 8) mg.o[warp][r][i * 8 + g] = x;
+      }
     }
   }
 };
@@ -1415,9 +1399,9 @@ Variant f32_rows() {
           F32Shape<R, DP>::kSmem, size_t(part_floats<R, DP>()) * sizeof(float)};
 }
 
-template <typename T, int V, int DP>
+template <typename T, int DP>
 Variant fma_rows() {
-  using Core = Fma<T, V, DP>;
+  using Core = Fma<T, DP>;
   return {reinterpret_cast<const void*>(&paged_attn_fma_kernel<T, Core>),
           reinterpret_cast<const void*>(&paged_attn_join_kernel<T, Core::kRows, DP>), Core::kRows, kThreads, false, sizeof(T),
           sizeof(Merge<kWarps, Core::kRows, DP>), size_t(part_floats<Core::kRows, DP>()) * sizeof(float)};
@@ -1444,9 +1428,9 @@ struct Variants {
     TcVariants<hf>::fill(v + 10);
     v[20] = f32_rows<4, 64>(), v[21] = f32_rows<4, 128>(), v[22] = f32_rows<4, 256>();
     v[23] = f32_rows<8, 64>(), v[24] = f32_rows<8, 128>();
-    v[25] = fma_rows<float, 1, 128>(), v[26] = fma_rows<float, 1, 256>();
-    v[27] = fma_rows<bf, 1, 128>(), v[28] = fma_rows<bf, 1, 256>();
-    v[29] = fma_rows<hf, 1, 128>(), v[30] = fma_rows<hf, 1, 256>();
+    v[25] = fma_rows<float, 128>(), v[26] = fma_rows<float, 256>();
+    v[27] = fma_rows<bf, 128>(), v[28] = fma_rows<bf, 256>();
+    v[29] = fma_rows<hf, 128>(), v[30] = fma_rows<hf, 256>();
   }
 };
 const Variant& variant_at(int i) {

@@ -268,6 +268,8 @@ def rope_append(cache: PagedCache, layer: int, q: torch.Tensor, k: torch.Tensor,
     n, heads, _ = q.shape
     dev, dt, dim = ctx.device, cache.dtype, cache.head_dim
     kv = (n, cache.n_kv_heads, dim)
+    if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
+        raise ValueError("k and v must be CUDA tensors")
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     if not (q.dtype is dt and k.dtype is dt and v.dtype is dt and q.shape[2] == dim and k.shape == kv and v.shape == kv
             and qs[2] == 1 and ks[2] == 1 and vs[2] == 1 and q.get_device() == dev and k.get_device() == dev
@@ -393,6 +395,9 @@ def verify_tokens(ctx: Context, logits: torch.Tensor, drafts: torch.Tensor, unif
         _on(ctx, logits, "logits")
         raise ValueError("logits must be float32, bfloat16 or float16 [n_seqs, n_draft + 1, vocab], contiguous within a row")
     x = _index(ctx, drafts, "drafts", (S, N - 1))
+    for t in (uniforms, temperature) if draft_probs is None else (uniforms, temperature, draft_probs):
+        if not isinstance(t, torch.Tensor):
+            raise ValueError("uniforms, temperature and draft_probs must be CUDA tensors")
     if not (uniforms.dtype is torch.float64 and uniforms.shape == (S, N) and uniforms.get_device() == dev
             and uniforms.is_contiguous()):
         raise ValueError(f"uniforms must be contiguous float64 [{S}, {N}] on device {dev}")

@@ -426,7 +426,8 @@ VC_API vc_status vc_rope_append(vc_ctx* ctx, const vc_kv_desc* cache, int32_t la
  * With n = seq_lens_dev[s] cached rows, the new tokens' own among them, token j
  * (n <= 0: a padding row of the batch) sees rows p < n - n_new + 1 + j:
  *   out[s][j][h] = sum_p softmax_p(scale * q[s][j][h] . k_p) v_p
- * over the rows of KV head h / (n_heads / n_kv_heads); lse_dev[s][j][h] (NULL:
+ * over the rows of KV head h / (n_heads / n_kv_heads) (a block table addresses at
+ * most 2^30 rows a sequence, VC_ENOTSUP otherwise); lse_dev[s][j][h] (NULL:
  * not wanted) = log sum_p exp(scale * q . k_p).  A token that sees no row gets
  * zeros and -infinity; rows a token does not see cannot reach its output,
  * whatever they hold.  Scores, sums and outputs are accumulated in f32 and

@@ -582,6 +582,11 @@ def test_decode_refusals(ctx):
                           cache.block_tables)
     with pytest.raises(ValueError):
         D.rope_append(shared, 0, x, x, x, pos, rope)
+    endless = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16, device="cuda").expand(1, (1 << 30) + 1, 1, 64)
+    with pytest.raises(Exception, match="2\\^30"):
+        D.paged_attention(D.PagedCache(ctx, [endless], [endless], pos[:1, None].contiguous()), 0, q[:1, :, :1], n[:1])
+    with pytest.raises(ValueError):
+        D.rope_append(cache, 0, x, None, x, pos, rope)
     odd = torch.zeros(2, 16, 1, 7, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(Exception):
         D.paged_attention(D.PagedCache(ctx, [odd], [odd], cache.block_tables), 0, odd[:2, :1, :1], n)

@@ -295,6 +295,7 @@ def test_verify_refusals(ctx):
                 dict(l=logits[:, :, :0]), dict(d=d.long()), dict(d=d[:, :1]), dict(u=uu.float()), dict(u=uu[:, :2]),
                 dict(t=tt.double()), dict(t=tt[:1]), dict(p=probs.double()), dict(p=probs[:, :1]),
                 dict(p=probs.transpose(1, 2).contiguous().transpose(1, 2)),
+                dict(u=None), dict(t=u), dict(d=None), dict(p=drafts),
                 dict(w=torch.empty(8, dtype=torch.uint8, device="cuda"))):
         kw = dict(l=logits, d=d, u=uu, t=tt, p=probs, w=None)
         kw.update(bad)
