@@ -86,11 +86,12 @@ __device__ __forceinline__ int64_t chunk_of(int64_t total, int n_ranges) {
   return (total + n_ranges - 1) / n_ranges;
 }
 
-// The sequence that holds tile `range * chunk`, found by the whole block.
+// The sequence that holds tile `range * chunk`, found by the whole block.  The second
+// pass has its own running sum: a warp may still be reading the first pass's total.
 template <int W>
 __device__ Place locate(const AttnArgs& a, int range) {
   __shared__ int64_t warp_sum[W];
-  __shared__ int64_t found_base, found_total;
+  __shared__ int64_t found_base, found_total, passed;
   __shared__ int found_seq;
   int64_t v0 = 0, incl0 = 0, base = 0;
   for (int c = 0; c < a.n_seqs; c += (W * 32)) {
@@ -119,9 +120,9 @@ __device__ Place locate(const AttnArgs& a, int range) {
       found_base = incl - v;
     }
     if (c + (W * 32) < a.n_seqs) {
-      if (threadIdx.x == (W * 32) - 1) found_total = incl;
+      if (threadIdx.x == (W * 32) - 1) passed = incl;
       __syncthreads();
-      base = found_total;
+      base = passed;
       __syncthreads();
     }
   }

@@ -1,0 +1,53 @@
+"""The decode step's operators at their edges: batches wider than a block, every attention kernel, masks of the lowest
+value, weights of few bits, arguments that overlap.  References and tolerances are those of ``test_gpu_decode``
+and ``test_gpu_verify`` where nothing else is said."""
+import numpy as np
+import pytest
+import torch
+
+from tests import test_gpu_decode as base
+from commitllm_b200 import decode as D
+
+pytestmark = pytest.mark.gpu
+
+DT = base.DT
+
+
+# ------------------------------------------------- batches wider than a block
+
+# (dtype, query heads, KV heads, new tokens, head size): one of each worker kernel, whose blocks scan the lengths of
+# 128 (4 warps), 128 and 192 sequences at a time
+WORKERS = [("bf16", 2, 1, 1, 64), ("f16", 6, 1, 4, 64), ("bf16", 8, 1, 5, 64), ("f32", 2, 1, 1, 64), ("bf16", 2, 1, 1, 66)]
+
+
+@pytest.mark.parametrize("S", [128, 129, 192, 193, 256, 400])
+@pytest.mark.parametrize("dtype,heads,kv,new,dim", WORKERS)
+def test_attention_batches_wider_than_a_block(ctx, dtype, heads, kv, new, dim, S):
+    rng = np.random.default_rng(S)
+    lens = [int(x) for x in rng.integers(0, 150, S)]
+    lens[1] = 0
+    lens[-1] = 149                    # the last sequence has tiles
+    cache, g = base.make_cache(ctx, S + dim, lens, kv, dim, 16, DT[dtype])
+    q = base.queries(g, S, new, heads, dim, DT[dtype])
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = D.paged_attention(cache, 0, q, n)
+    ctx.sync(60000)
+    # the same sequences in batches that one pass over the lengths covers.  Their ranges are cut elsewhere, so the
+    # sums run in another order: each side is within the reference's tolerance of the 64-bit values
+    some = sorted(set([0, 1, 126, 127, S - 2, S - 1] + [x for x in (128, 191, 192, 255, 256) if x < S]))
+    small = D.PagedCache(ctx, cache.k_layers, cache.v_layers, cache.block_tables[some].contiguous())
+    ro, _, to, _ = base.reference(small, 0, q[some], [lens[s] for s in some])
+    sub = torch.finfo(q.dtype).smallest_normal
+    assert bool(((out[some].double() - ro).abs() <= to + sub).all())
+    for a in range(0, S, 100):
+        part = D.PagedCache(ctx, cache.k_layers, cache.v_layers, cache.block_tables[a:a + 100].contiguous())
+        got = D.paged_attention(part, 0, q[a:a + 100], n[a:a + 100])
+        ctx.sync(60000)
+        # both within rel * (weighted mean of |v|) <= rel * max |v| and their rounding: rel as in the reference, with
+        # scores of at most 150 keys
+        e = torch.finfo(q.dtype).eps
+        vmax = float(cache.v_layers[0].abs().max())
+        kmax = float(cache.k_layers[0].abs().sum(-1).max()) * float(q.abs().max()) * dim ** -0.5
+        rel = 2 * (dim + 4) * 2.0 ** -24 * kmax + 2.0 ** -21 + 2.0 ** -16 + 300 * 2.0 ** -24
+        diff = (got.double() - out[a:a + 100].double()).abs()
+        assert bool((diff <= 2 * rel * vmax + e * got.double().abs() + e * rel * vmax + sub).all())
