@@ -27,6 +27,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cfloat>
+
 #include "vc_internal.h"
 
 namespace cg = cooperative_groups;
@@ -434,7 +436,8 @@ __global__ void __launch_bounds__(kPickThreads, 1) verify_pick_kernel(const __gr
   auto set_row = [&](int i, float m) {
     w.l = static_cast<const T*>(a.logits) + seq * a.logits_seq + i * a.logits_tok;
     w.m = double(m);
-    w.none = fmaxf(__fadd_ru(m, __fmul_rn(temp, -744.44f)), -3.4e38f);
+    // never above the lowest finite value: a row may consist of it, and only -infinity rules out
+    w.none = fmaxf(__fadd_ru(m, __fmul_rn(temp, -744.44f)), -FLT_MAX);
   };
   auto probs_row = [&](int i) { return a.draft_probs + seq * a.probs_seq + i * a.probs_tok; };
   __syncthreads();
