@@ -28,6 +28,7 @@
 #include <cuda_fp16.h>
 
 #include <cfloat>
+#include <cmath>
 
 #include "vc_internal.h"
 
@@ -49,6 +50,10 @@ static_assert(32 * sizeof(VerifyPart) <= kVerifyRowBytes, "a row's slices fit it
 // of the maximum by 2^-21 each; 126 * 3 * 2^-24 * ln 2 + 2^-22 + 2^-17 + 12 * 2^-21
 // < 3e-5.
 constexpr double kOpen = 4e-5;
+// That holds for temperatures in [1e-30, 1e30]: log2(e) / T is then a normal number, and
+// a difference of two logits that passes f32 weighs nothing.  At any other temperature
+// every test is open.
+__device__ __forceinline__ double open_part(float t) { return t >= 1e-30f && t <= 1e30f ? kOpen : double(INFINITY); }
 
 template <typename T> __device__ __forceinline__ float to_f32(T x);
 template <> __device__ __forceinline__ float to_f32<float>(float x) { return x; }
@@ -425,6 +430,7 @@ __global__ void __launch_bounds__(kPickThreads, 1) verify_pick_kernel(const __gr
   sl.per_warp = ((per_cta + kPickWarps - 1) / kPickWarps + 7) / 8 * 8;
   const float temp = a.temperature[seq];
   const bool greedy = !(temp > 0.f);
+  const double open = open_part(temp);
   const double* u = a.uniforms + int64_t(seq) * (a.n_draft + 1);
   const int32_t* drafts = a.drafts + int64_t(seq) * a.n_draft;
   int32_t* out = a.tokens + int64_t(seq) * (a.n_draft + 1);
@@ -517,7 +523,7 @@ __global__ void __launch_bounds__(kPickThreads, 1) verify_pick_kernel(const __gr
     w.q = nullptr;
     w.wide = a.wide_logits;
     if (!a.draft_probs) {
-      const double goal = u[i] * r.s, edge = kOpen * r.s;
+      const double goal = u[i] * r.s, edge = open * r.s;
       const bool in = goal > r.b + edge && goal < r.b + r.wx - edge;
       const bool off = goal < r.b - edge || goal > r.b + r.wx + edge;
       if (r.there && in) continue;                  // kept, whatever the rounding
@@ -541,7 +547,7 @@ __global__ void __launch_bounds__(kPickThreads, 1) verify_pick_kernel(const __gr
     if (r.there) {
       const double want = u[i] * double(r.qx), have = want * r.s;
       bool keep = have < r.wx;
-      if (!(fabs(have - r.wx) > kOpen * fmax(have, r.wx)) && have > 0.0) {
+      if (!(fabs(have - r.wx) > open * fmax(have, r.wx)) && have > 0.0) {
         total = total_of();
         have_total = true;
         keep = want < r.wx / total;

@@ -32,3 +32,26 @@ def test_verify_rows_of_the_lowest_value(ctx, dtype, V, with_probs):
         want, _ = base.plain(logits.double().cpu().numpy(), drafts, u, temperature)
         drafts[::2, 0] = want[::2, 0]
     base.check(ctx, logits, drafts, u, temperature, probs)
+
+
+@pytest.mark.parametrize("with_probs", [False, True])
+@pytest.mark.parametrize("t", [1e-45, 1e-42, 3e-39, 1e-36, 1e30, 1e34, 1e36, 1e37, 1e38, 3e38])
+def test_verify_temperatures_at_the_types_ends(ctx, t, with_probs):
+    """Logits that differ by a few temperatures, however small or large that is."""
+    S, k, V = 32, 2, 3001
+    rng = np.random.default_rng(23)
+    t = float(np.float32(t))
+    spread = min(4.0 * t, 3.3e38)
+    l = np.clip(rng.uniform(-spread, spread, (S, k + 1, V)), -3.4e38, 3.4e38).astype(np.float32)
+    l[:, :, 1::7] = np.finfo(np.float32).min
+    u = rng.random((S, k + 1))
+    temperature = np.full(S, t, np.float32)
+    logits = torch.tensor(l, device="cuda")
+    drafts = rng.integers(0, V, (S, k)).astype(np.int32)
+    probs = None
+    if with_probs:
+        probs = torch.softmax(torch.tensor(rng.standard_normal((S, k, V)).astype(np.float32), device="cuda"), -1)
+    else:
+        want, _ = base.plain(l.astype(np.float64), drafts, u, temperature)
+        drafts[::2, 0] = want[::2, 0]
+    base.check(ctx, logits, drafts, u, temperature, probs)
