@@ -12,6 +12,7 @@
 #include <mutex>
 #include <string>
 #include <thread>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -1324,8 +1325,17 @@ struct Slot {
   }
 };
 
+// Whether a slot holds a value of the argument's type: 32-bit integers have to fit.
+template <typename A>
+bool slot_fits(int64_t v) {
+  return !std::is_same<A, int32_t>::value || v == int64_t(int32_t(v));
+}
+
 template <typename... A, size_t... I>
 vc_status call_slots(vc_status (*fn)(A...), const int64_t* s, std::index_sequence<I...>) {
+  const bool fits[] = {slot_fits<A>(s[I])...};
+  for (size_t i = 0; i < sizeof...(A); ++i)
+    if (!fits[i]) return fail(VC_EINVAL, "vc_decode_call: slot %zu, %lld, does not fit 32 bits", i, static_cast<long long>(s[i]));
   return fn(static_cast<A>(Slot{s[I]})...);
 }
 

@@ -488,7 +488,8 @@ VC_API vc_status vc_verify_tokens_workspace(vc_ctx* ctx, int32_t n_seqs, int32_t
  * The decode-step calls with their arguments, the context first, in 64-bit slots
  * in the order declared: pointers and integers as they are, doubles as their bits.
  * For bindings that pay for each argument (a ctypes call of vc_rope_append's 23
- * takes 2.6 us, this one 0.4).  VC_EINVAL where n_slots is not the call's number.
+ * takes 2.6 us, this one 0.4).  VC_EINVAL where n_slots is not the call's number, or a
+ * 32-bit argument's slot holds a value that does not fit 32 bits.
  */
 #define VC_CALL_ROPE_APPEND 0
 #define VC_CALL_PAGED_ATTENTION 1

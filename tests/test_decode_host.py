@@ -1,6 +1,7 @@
 """Host side of the decode-step operators: rope frequencies, and refusals that need no GPU."""
 import ctypes
 import math
+import struct
 
 import numpy as np
 import pytest
@@ -61,3 +62,37 @@ def test_entry_points_refuse_null_arguments():
     assert lib.vc_decode_call(1, 15, bytes(120)) == _lib.VC_EINVAL
     assert lib.vc_decode_call(1, 16, bytes(128)) == _lib.VC_EINVAL
     assert lib.vc_verify_tokens_workspace(None, 0, 0, 0, ctypes.byref(out)) == _lib.VC_EINVAL
+
+
+def packed_call(which, values):
+    """A vc_decode_call of these arguments (ints, floats), the context a block of zeros that no check reads."""
+    lib = _lib.lib()
+    ctx = ctypes.create_string_buffer(4096)
+    slots = struct.pack("q" * (len(values) + 1), ctypes.addressof(ctx),
+                        *(v if isinstance(v, int) else struct.unpack("q", struct.pack("d", v))[0] for v in values))
+    return lib.vc_decode_call(which, len(values) + 1, slots)
+
+
+def test_packed_arguments_past_32_bits_are_refused():
+    """32-bit arguments in 64-bit slots: a value that does not fit is an error, not its low half.  Empty calls, which
+    return before they touch a GPU."""
+    ptrs = (ctypes.c_void_p * 1)(256)
+    d = _lib.KvDesc()
+    d.n_layers = d.n_kv_heads = 1
+    d.head_dim, d.dtype, d.n_seqs, d.block_size, d.max_blocks_per_seq = 64, _lib.VC_DTYPE_BF16, 2, 16, 4
+    d.stride_page, d.stride_row, d.stride_head, d.cache_elems, d.block_tables = 1024, 64, 64, 8192, 256
+    d.k_layers = d.v_layers = ctypes.cast(ptrs, ctypes.POINTER(ctypes.c_void_p))
+    desc = ctypes.addressof(d)
+    rope = [desc, 0, 0, 256, 0, 1, 256, 64, 64, 256, 64, 64, 256, 64, 64, 256, 64, 64, 256, 64, 1.0, 0]
+    attend = [desc, 0, 0, 1, 1, 256, 64, 64, 64, 256, 0.125, 256, 0, 256, 1 << 20]
+    verify = [0, 1, 100, 256, _lib.VC_DTYPE_F32, 200, 100, 0, 0, 0, 256, 256, 256, 256, 256, 256, 1 << 20]
+    for which, good, narrow in ((_lib.VC_CALL_ROPE_APPEND, rope, (1, 2, 5, 19, 21)),
+                                (_lib.VC_CALL_PAGED_ATTENTION, attend, (1, 2, 3, 4)),
+                                (_lib.VC_CALL_VERIFY_TOKENS, verify, (0, 1, 2, 4))):
+        assert packed_call(which, good) == _lib.VC_OK
+        for at in narrow:
+            for off in (1 << 32, -(1 << 32), 1 << 40):
+                bad = list(good)
+                bad[at] += off
+                assert packed_call(which, bad) == _lib.VC_EINVAL, (which, at, off)
+                assert "32 bits" in _lib.last_error()

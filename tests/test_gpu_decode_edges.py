@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from tests import test_gpu_decode as base
+from commitllm_b200 import commit as C
 from commitllm_b200 import decode as D
 
 pytestmark = pytest.mark.gpu
@@ -51,3 +52,20 @@ def test_attention_batches_wider_than_a_block(ctx, dtype, heads, kv, new, dim, S
         rel = 2 * (dim + 4) * 2.0 ** -24 * kmax + 2.0 ** -21 + 2.0 ** -16 + 300 * 2.0 ** -24
         diff = (got.double() - out[a:a + 100].double()).abs()
         assert bool((diff <= 2 * rel * vmax + e * got.double().abs() + e * rel * vmax + sub).all())
+
+
+# ------------------------------------------------------------------ refusals
+
+
+@pytest.mark.parametrize("layer", [2 ** 32, -2 ** 32, 2 ** 31, 2 ** 40])
+def test_layers_past_32_bits_are_refused(ctx, layer):
+    cache, g = base.make_cache(ctx, 51, [32, 32], 2, 64, 16, torch.bfloat16)
+    before = [t.clone() for t in (cache.k_layers[0], cache.v_layers[0])]
+    x = torch.randn(2, 2, 64, generator=g, device="cuda").to(torch.bfloat16)
+    pos = torch.ones(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        D.rope_append(cache, layer, x, x, x, pos, D.rope_table(ctx, C.RopeConfig(), 64))
+    with pytest.raises(ValueError):
+        D.paged_attention(cache, layer, x[:, None].contiguous(), pos)
+    ctx.sync(60000)
+    assert torch.equal(before[0], cache.k_layers[0]) and torch.equal(before[1], cache.v_layers[0])
