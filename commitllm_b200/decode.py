@@ -125,6 +125,8 @@ class PagedCache:
         self.dtype = k0.dtype
         self.n_pages, self.block_size, self.n_kv_heads, self.head_dim = (int(x) for x in k0.shape)
         self.n_seqs, self.max_blocks = (int(x) for x in block_tables.shape)
+        if max(self.n_layers, *k0.shape[1:], *block_tables.shape) >= 1 << 31:      # the descriptor's integers
+            raise ValueError("layers, block_size, n_kv_heads, head_dim, n_seqs and max_blocks must be below 2^31")
         d = KvDesc()
         d.n_layers, d.n_kv_heads, d.head_dim = self.n_layers, self.n_kv_heads, self.head_dim
         d.dtype, d.n_seqs = _CACHE_DTYPES[k0.dtype], self.n_seqs

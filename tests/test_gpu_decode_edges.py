@@ -69,3 +69,12 @@ def test_layers_past_32_bits_are_refused(ctx, layer):
         D.paged_attention(cache, layer, x[:, None].contiguous(), pos)
     ctx.sync(60000)
     assert torch.equal(before[0], cache.k_layers[0]) and torch.equal(before[1], cache.v_layers[0])
+
+
+def test_cache_sizes_past_32_bits_are_refused(ctx):
+    one = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    D.PagedCache(ctx, [one], [one], table)
+    for shape in ((1, 2 ** 32 + 16, 1, 64), (1, 1, 2 ** 32 + 1, 64), (1, 2 ** 31, 1, 64)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            D.PagedCache(ctx, [one.expand(shape)], [one.expand(shape)], table)
