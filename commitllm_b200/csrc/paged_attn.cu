@@ -194,6 +194,14 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// ln(2^m * l).  The power of two in l goes to m first: a reference far below the maximum
+// makes both large, and their sum is not.
+__device__ __forceinline__ float log_sum(float m, float l) {
+  int k;
+  const float f = frexpf(l, &k);
+  return ((m + float(k)) + log2f(f)) * 0.6931471805599453f;
+}
+
 // Weights are taken relative to a reference that is at most 2^8 below the largest one
 // seen: it follows the maximum only when that has grown by more, so the sums so far are
 // seldom rescaled (a maximum of random scores grows in half of the first 30 tiles) and
@@ -250,7 +258,7 @@ __device__ __noinline__ void emit(const AttnArgs& a, Merge<W, R, D>& mg, Target 
         if (to.row0 + r < a.rows) {
           const RowAt ra = row_at(a, to.seq, to.kvh, to.row0 + r);
           at = ra.out * a.head_dim;
-          if (a.lse) a.lse[ra.out] = l == 0.f ? ninf() : (top + log2f(l)) * 0.6931471805599453f;
+          if (a.lse) a.lse[ra.out] = l == 0.f ? ninf() : log_sum(top, l);
         }
       }
 #pragma unroll
@@ -295,9 +303,12 @@ __device__ __noinline__ void emit(const AttnArgs& a, Merge<W, R, D>& mg, Target 
 
 // ------------------------------------------- 16-bit rows: tensor-core variant
 
+// kLift: weights reach 2^(kLift + kSlack), and a reference comes down again where a row's
+// tile lies below 2^-kLift of it (weigh; 0: it only rises).
 template <typename T> struct Bits;
 template <> struct Bits<__nv_bfloat16> {
   static constexpr uint32_t kExp = 0x7F80;
+  static constexpr float kLift = 0.f;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
@@ -314,6 +325,7 @@ template <> struct Bits<__nv_bfloat16> {
 };
 template <> struct Bits<__half> {
   static constexpr uint32_t kExp = 0x7C00;
+  static constexpr float kLift = 7.f;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
@@ -390,6 +402,17 @@ __device__ __forceinline__ void pv_of_token(float (&o)[4], const uint32_t (&vf)[
 // reference moves, and the weights in two 16-bit parts.  A lane compares only its own
 // scores with the reference; the row's maximum is exchanged where one of them passes
 // it.  scale is not negative.
+//
+// A 16-bit number has 11 bits only down to 2^-14 in f16, and nothing below 2^-24.  Next to
+// a key that takes almost all of the softmax, the others' weights would be lost from the
+// products while the f32 sum still counted them: with a value of zero at that key
+// they are the whole output.  So f16 weights are taken relative to 2^-kLift of the
+// largest (2^15 is then the most that occurs), and where a row's scores of the tile all lie
+// another 2^kLift lower the reference follows them down: every tile's largest weight is
+// at least 2^-7 and its two parts' error, 2^-25 at most, 2^-18 of it.  The sums are
+// f32 and may grow with that: to 2^kRoom for a row's weights, 2^96 for its outputs.  The
+// test costs 1 % where instructions bound (35 rows over 159 MB: 62.2 -> 62.9 us).
+constexpr float kRoom = 80.f;
 template <typename B, int NB, int KS>
 __device__ __forceinline__ void weigh(float (&s)[NB][2][2], float scale, bool all_seen, int left, int c, float& m, float& l,
                                       float (&o)[KS][4], uint32_t (&hi)[NB][2], uint32_t (&lo)[NB][2]) {
@@ -406,12 +429,26 @@ __device__ __forceinline__ void weigh(float (&s)[NB][2][2], float scale, bool al
 #pragma unroll
   for (int b = 0; b < NB; ++b) top = fmaxf(top, fmaxf(fmaxf(s[b][0][0], s[b][0][1]), fmaxf(s[b][1][0], s[b][1][1])));
   top = top == ninf() ? top : top * scale;       // (-infinity * 0)
-  if (__any_sync(~0u, top > m + kSlack)) {
-    // what is summed so far shrinks to the new maximum
+  bool move = __any_sync(~0u, top > m + (kSlack + B::kLift));
+  if constexpr (B::kLift > 0) {
+    unsigned low = __ballot_sync(~0u, top < m - B::kLift);      // by lane; then of a row's four
+    low &= low >> 1;
+    low &= low >> 2;
+    move = move || (low & 0x11111111u);
+  }
+  if (move) {
+    // what is summed so far shrinks to the new maximum, or grows
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-    top = fmaxf(top, m);
-    const float f = m == ninf() ? 0.f : ex2(m - top);
+    float to = fmaxf(top - B::kLift, m);
+    if constexpr (B::kLift > 0) {
+      float sum = l + __shfl_xor_sync(~0u, l, 1);
+      sum += __shfl_xor_sync(~0u, sum, 2);
+      // (the sum's exponent, rounded up)
+      const float least = m + (float((__float_as_int(sum) >> 23) - 126) - kRoom);
+      if (top < m - B::kLift && top > ninf()) to = fminf(fmaxf(top - B::kLift, least), m);
+    }
+    const float f = m == ninf() ? 0.f : ex2(m - to);
     l *= f;
     const float f0 = __shfl_sync(~0u, f, c * 8), f1 = __shfl_sync(~0u, f, c * 8 + 4);
 #pragma unroll
@@ -419,7 +456,7 @@ __device__ __forceinline__ void weigh(float (&s)[NB][2][2], float scale, bool al
       o[i][0] *= f0, o[i][2] *= f0;
       o[i][1] *= f1, o[i][3] *= f1;
     }
-    m = top;
+    m = to;
   }
   const float ref = m == ninf() ? 0.f : m;
 #pragma unroll
@@ -454,9 +491,8 @@ __device__ __forceinline__ void weigh(float (&s)[NB][2][2], float scale, bool al
 // fragment without any exchange, and ldmatrix.trans gives V^T.
 //
 // P is rounded to 16 bits twice (its value, then what that left over), so the
-// products see 16 (bf16) or more bits of it (f16: of weights under 2^-14 of the
-// largest, 2^-25 of that) and the output keeps the error of its own rounding; the row
-// sums are taken in f32.
+// products see 16 (bf16) or more bits of it (f16: see weigh) and the output keeps the
+// error of its own rounding; the row sums are taken in f32.
 //
 // Measured: 1.34 GB (64 sequences of up to 8192 rows, 8 KV heads of 128) in 198 us and
 // 1.07 GB (2 of 131072) in 164 us, 6.6 - 6.8 TB/s; DRAM 81 %, tensor pipe 21 % busy.
@@ -1364,7 +1400,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __g
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   for (int d = threadIdx.x; d < a.head_dim; d += kJoinThreads)
     out[d] = from_f32<T>((f[0] * acc[0][d] + f[1] * acc[1][d] + f[2] * acc[2][d] + f[3] * acc[3][d]) * inv);
-  if (threadIdx.x == 0 && a.lse) a.lse[at.out] = l == 0.f ? ninf() : (top + log2f(l)) * 0.6931471805599453f;
+  if (threadIdx.x == 0 && a.lse) a.lse[at.out] = l == 0.f ? ninf() : log_sum(top, l);
 }
 
 // ------------------------------------------------------------------ variants

@@ -54,6 +54,69 @@ def test_attention_batches_wider_than_a_block(ctx, dtype, heads, kv, new, dim, S
         assert bool((diff <= 2 * rel * vmax + e * got.double().abs() + e * rel * vmax + sub).all())
 
 
+# -------------------------------------------------------- weights of few bits
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("heads,kv,new,dim", [(64, 64, 1, 64), (32, 32, 1, 128), (48, 4, 1, 128), (96, 4, 1, 64), (160, 4, 1, 128)])
+def test_attention_small_weights_next_to_a_large_one(ctx, dtype, heads, kv, new, dim):
+    """A key that takes almost all of the softmax and whose value is zero, and keys 15 - 20 nats below it: the output
+    is theirs alone.
+
+    Tolerance: the reference's, and what two 16-bit numbers leave of a weight.  The kernel's f16 weights are relative to
+    a reference that the large key, the first one, sets to 2^-7 of itself, or that has come down to 2^-7 of the largest
+    of a warp's 16 or 32 keys; rounding to a multiple of 2^-24 is off by at most 2^-25, so by 2^-32 of the large
+    key's weight among its neighbours, and by 2^-18 of the largest weight among its own 32 keys elsewhere.
+    """
+    dt, S, L = DT[dtype], 8, 2048
+    cache, g = base.make_cache(ctx, heads + dim, [L] * S, kv, dim, 16, dt, fill=0.0)
+    k, v = cache.k_layers[0], cache.v_layers[0]
+    # the score of a key is its first element
+    k[..., 0] = (torch.rand(k.shape[:-1], generator=g, device="cuda") * 5).to(dt)
+    v.copy_(torch.rand(v.shape, generator=g, device="cuda") * 1000 + 500)
+    for s in range(S):
+        k[int(cache.block_tables[s, 0]), 0, :, 0] = 20.0
+        v[int(cache.block_tables[s, 0]), 0] = 0.0
+    q = torch.zeros(S, new, heads, dim, dtype=dt, device="cuda")
+    q[..., 0] = 1.0
+    lens = [L] * S
+    lens[3] = 700
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = D.paged_attention(cache, 0, q, n, scale=1.0)
+    ctx.sync(60000)
+    few = [0, 3]
+    small = D.PagedCache(ctx, [k], [v], cache.block_tables[few].contiguous())
+    ro, _, to, _ = base.reference(small, 0, q[few], [lens[s] for s in few], scale=1.0)
+    for i, s in enumerate(few):
+        kk, vv = base.rows_of(small, 0, i, lens[s])
+        p = torch.softmax(kk[:, :, 0], 0)                                  # [keys, kv heads]
+        pad = -len(p) % 32
+        top = torch.nn.functional.pad(p, (0, 0, 0, pad)).view(-1, 32, kv).amax(1).repeat_interleave(32, 0)[:len(p)]
+        unit = 2.0 ** -18 * top
+        unit[:32] = 2.0 ** -32 * p[0]
+        extra = torch.einsum("ng,ngd->gd", unit, vv.abs()).repeat_interleave(heads // kv, 0)
+        assert float(ro[i].abs().min()) > 1e-3                             # well above f16's smallest numbers
+        assert bool(((out[s].double() - ro[i]).abs() <= to[i] + extra).all()), float(((out[s].double() - ro[i]) / ro[i]).abs().max())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("heads,kv,dim", [(16, 16, 128), (40, 2, 128)])
+def test_attention_scores_that_rise_and_fall(ctx, dtype, heads, kv, dim):
+    """Runs of 64 keys by turns 40 nats above and below each other, falling all the way, and rising all the way."""
+    dt, S, L = DT[dtype], 3, 1600
+    cache, g = base.make_cache(ctx, heads, [L] * S, kv, dim, 16, dt)
+    k = cache.k_layers[0]
+    run = torch.arange(L, device="cuda") // 64
+    level = [run % 2 * 40.0, -3.0 * run, 3.0 * run]
+    for s in range(S):
+        p = torch.arange(L, device="cuda")
+        page = cache.block_tables[s].long()[p // 16]
+        k[page, p % 16] = 0.0
+        k[page, p % 16, :, 0] = (level[s][:, None] + torch.rand(L, kv, generator=g, device="cuda")).to(dt)
+    q = torch.zeros(S, 1, heads, dim, dtype=dt, device="cuda")
+    q[..., 0] = 1.0
+    base.check_attention(ctx, cache, q, [L, L, L - 5], scale=1.0)
+
+
 # ------------------------------------------------------------------ refusals
 
 
