@@ -1100,6 +1100,23 @@ vc_status check_rows(const void* p, int esz, const char* fn, const char* name) {
   return VC_OK;
 }
 
+// Whether any two of n1 x n2 rows of `len` elements, at strides s1 and s2, share an element.
+bool rows_overlap(int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t len) {
+  using Wide = __int128;                    // strides are the caller's: no product overflows
+  const Wide a = s1 < 0 ? -Wide(s1) : s1, b = s2 < 0 ? -Wide(s2) : s2;
+  if ((n1 > 1 && a < len) || (n2 > 1 && b < len)) return true;
+  if (n1 < 2 || n2 < 2) return false;
+  // the rows of one dimension inside a stride of the other
+  if (b >= (n1 - 1) * a + len || a >= (n2 - 1) * b + len) return false;
+  // interleaved: for each i, the j that bring row (i, j) nearest to row (0, 0), either way
+  for (int64_t i = 1; i < n1; ++i)
+    for (Wide j = i * a / b; j <= i * a / b + 1; ++j) {
+      const Wide gap = i * a - j * b;
+      if (j < n2 && (gap < 0 ? -gap : gap) < len) return true;
+    }
+  return false;
+}
+
 vc_status check_attn(const vc_kv_desc* d, int32_t layer, int32_t n_new, int32_t n_heads, const char* fn) {
   vc_status r = check_paged(d, layer, fn);
   if (r) return r;
@@ -1147,6 +1164,10 @@ vc_status vc_rope_append(vc_ctx* c, const vc_kv_desc* d, int32_t layer, int32_t 
     return fail(VC_EINVAL, "vc_rope_append: rotary_dim %d is odd or not in [2, head_dim]", rotary_dim);
   if ((d->n_kv_heads > 1 && d->stride_head < d->head_dim) || (d->block_size > 1 && d->stride_row < d->head_dim))
     return fail(VC_EINVAL, "vc_rope_append: the cache's rows or heads overlap");
+  if (d->k_layers[layer] == d->v_layers[layer])
+    return fail(VC_EINVAL, "vc_rope_append: the K and V rows of layer %d overlap", layer);
+  if (rows_overlap(n_heads, qo_head, n_tokens, qo_tok, d->head_dim))
+    return fail(VC_EINVAL, "vc_rope_append: the rows of q_out overlap");
   if (!seq_ids && n_tokens > d->n_seqs)
     return fail(VC_EINVAL, "vc_rope_append: %d tokens of %d sequences need seq_ids", n_tokens, d->n_seqs);
   if (n_tokens == 0) return VC_OK;

@@ -260,7 +260,8 @@ def rope_append(cache: PagedCache, layer: int, q: torch.Tensor, k: torch.Tensor,
     the token's sequence (default: token t is sequence t's).  The first
     ``rope.rotary_dim`` elements of each head are rotated, in halves ``(i, i +
     rotary_dim/2)`` or, ``interleaved``, in neighbours ``(2i, 2i+1)``.  Returns
-    the rotated queries (``q_out``, which may be ``q``; new by default).  Two
+    the rotated queries (``q_out``, which may be ``q`` and otherwise overlaps no
+    input; its rows may not overlap, nor a layer's K and V; new by default).  Two
     tokens of a call must not share a row.  A position or page outside the
     cache is raised by the next ``ctx.sync()``.
     """

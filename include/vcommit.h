@@ -411,7 +411,8 @@ VC_API vc_status vc_kv_transcript_commit(vc_ctx* ctx, const vc_kvt_desc* desc, i
  * `factor`; elements from rotary_dim on are kept.  q goes to q_out (which may
  * be q itself), k and v to row p of the sequence.  p < 0 marks padding: q is
  * copied unchanged and no row is written.  Two tokens of one call must not
- * share a row: that row would hold a mix of both.
+ * share a row: that row would hold a mix of both.  VC_EINVAL where rows of q_out
+ * overlap, or the layer's K and V are one buffer; q_out overlaps no other input.
  */
 VC_API vc_status vc_rope_append(vc_ctx* ctx, const vc_kv_desc* cache, int32_t layer, int32_t n_tokens,
                                 const int32_t* positions_dev, const int32_t* seq_ids_dev, int32_t n_heads,

@@ -76,12 +76,12 @@ def packed_call(which, values):
 def test_packed_arguments_past_32_bits_are_refused():
     """32-bit arguments in 64-bit slots: a value that does not fit is an error, not its low half.  Empty calls, which
     return before they touch a GPU."""
-    ptrs = (ctypes.c_void_p * 1)(256)
+    k, v = (ctypes.c_void_p * 1)(256), (ctypes.c_void_p * 1)(512)
     d = _lib.KvDesc()
     d.n_layers = d.n_kv_heads = 1
     d.head_dim, d.dtype, d.n_seqs, d.block_size, d.max_blocks_per_seq = 64, _lib.VC_DTYPE_BF16, 2, 16, 4
     d.stride_page, d.stride_row, d.stride_head, d.cache_elems, d.block_tables = 1024, 64, 64, 8192, 256
-    d.k_layers = d.v_layers = ctypes.cast(ptrs, ctypes.POINTER(ctypes.c_void_p))
+    d.k_layers, d.v_layers = (ctypes.cast(p, ctypes.POINTER(ctypes.c_void_p)) for p in (k, v))
     desc = ctypes.addressof(d)
     rope = [desc, 0, 0, 256, 0, 1, 256, 64, 64, 256, 64, 64, 256, 64, 64, 256, 64, 64, 256, 64, 1.0, 0]
     attend = [desc, 0, 0, 1, 1, 256, 64, 64, 64, 256, 0.125, 256, 0, 256, 1 << 20]
@@ -96,3 +96,33 @@ def test_packed_arguments_past_32_bits_are_refused():
                 bad[at] += off
                 assert packed_call(which, bad) == _lib.VC_EINVAL, (which, at, off)
                 assert "32 bits" in _lib.last_error()
+
+
+def test_rope_append_refuses_outputs_that_overlap():
+    """Strides of q_out against every pair of rows, on the CPU: calls that pass the check stop at a NULL
+    position array."""
+    k, v = (ctypes.c_void_p * 1)(256), (ctypes.c_void_p * 1)(512)
+    d = _lib.KvDesc()
+    d.n_layers = d.n_kv_heads = 1
+    d.head_dim, d.dtype, d.n_seqs, d.block_size, d.max_blocks_per_seq = 4, _lib.VC_DTYPE_BF16, 8, 16, 4
+    d.stride_page, d.stride_row, d.stride_head, d.cache_elems, d.block_tables = 64, 4, 4, 512, 256
+    d.k_layers, d.v_layers = (ctypes.cast(p, ctypes.POINTER(ctypes.c_void_p)) for p in (k, v))
+    seen = set()
+    for heads in (1, 2, 3, 5):
+        for toks in (1, 2, 4):
+            for hs in (0, 2, 4, -4, 5, 6, 8, 12, 16, 2 ** 62):
+                for ts in (0, 3, 4, -8, 6, 8, 10, 12, 16, 20, -2 ** 63):
+                    rows = [range(h * hs + t * ts, h * hs + t * ts + 4) for h in range(heads) for t in range(toks)]
+                    starts = sorted(r.start for r in rows)
+                    want = any(b - a < 4 for a, b in zip(starts, starts[1:]))
+                    got = packed_call(_lib.VC_CALL_ROPE_APPEND,
+                                      [ctypes.addressof(d), 0, toks, 0, 0, heads, 256, 4, 4, 256, ts, hs, 256, 4, 4, 256, 4, 4,
+                                       256, 4, 1.0, 0])
+                    assert got == _lib.VC_EINVAL
+                    assert ("overlap" in _lib.last_error()) == want, (heads, toks, hs, ts)
+                    seen.add(want)
+    assert seen == {False, True}
+    d.v_layers = d.k_layers
+    assert packed_call(_lib.VC_CALL_ROPE_APPEND, [ctypes.addressof(d), 0, 1, 0, 0, 1, 256, 4, 4, 256, 4, 4, 256, 4, 4, 256, 4, 4,
+                                                  256, 4, 1.0, 0]) == _lib.VC_EINVAL
+    assert "overlap" in _lib.last_error()

@@ -141,3 +141,27 @@ def test_cache_sizes_past_32_bits_are_refused(ctx):
     for shape in ((1, 2 ** 32 + 16, 1, 64), (1, 1, 2 ** 32 + 1, 64), (1, 2 ** 31, 1, 64)):
         with pytest.raises(ValueError, match="2\\^31"):
             D.PagedCache(ctx, [one.expand(shape)], [one.expand(shape)], table)
+
+
+def test_rope_append_refuses_rows_that_overlap(ctx):
+    """Outputs that share memory among themselves: queries expanded over heads or tokens, K and V in one buffer."""
+    cache, g = base.make_cache(ctx, 50, [32, 32], 2, 64, 16, torch.bfloat16)
+    x = torch.randn(2, 2, 64, generator=g, device="cuda").to(torch.bfloat16)
+    pos = torch.zeros(2, dtype=torch.int32, device="cuda")
+    rope = D.rope_table(ctx, C.RopeConfig(), 64)
+    one = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    flat = torch.zeros(64 * 4, dtype=torch.bfloat16, device="cuda")
+    for bad in (one.expand(2, 2, 64), flat[:128].view(1, 2, 64).expand(2, -1, -1), flat[:128].view(2, 1, 64).expand(-1, 2, -1),
+                flat.as_strided((2, 2, 64), (128, 32, 1)), flat.as_strided((2, 2, 64), (32, 128, 1)),
+                flat.as_strided((2, 2, 64), (64, 64, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            D.rope_append(cache, 0, x, x, x, pos, rope, q_out=bad)
+    for good in (flat.as_strided((2, 2, 64), (64, 128, 1)), flat.view(2, 2, 64)):
+        D.rope_append(cache, 0, x, x, x, pos, rope, q_out=good)
+        ctx.sync(60000)
+        assert torch.equal(good, x)                       # position 0 turns nothing
+    same = D.PagedCache(ctx, [cache.k_layers[0]], [cache.k_layers[0]], cache.block_tables)
+    with pytest.raises(ValueError, match="overlap"):
+        D.rope_append(same, 0, x, x, x, pos, rope)
+    D.paged_attention(same, 0, x[:, None].contiguous(), pos)          # reading one buffer as both is fine
+    ctx.sync(60000)
