@@ -54,6 +54,58 @@ def test_attention_batches_wider_than_a_block(ctx, dtype, heads, kv, new, dim, S
         assert bool((diff <= 2 * rel * vmax + e * got.double().abs() + e * rel * vmax + sub).all())
 
 
+# ----------------------------------------------------- every attention kernel
+
+def kernel_of(dtype, rows, dim, wide):
+    """Number of the kernel that ``variant_for`` in csrc/paged_attn.cu takes for this call: the rule restated."""
+    size = 0 if dim <= 64 else 1 if dim <= 128 else 2
+    if not wide:
+        return {"f32": 25, "bf16": 27, "f16": 29}[dtype] + (size == 2)
+    if dtype == "f32":
+        return (23 if rows > 4 and size < 2 else 20) + size
+    first = 0 if dtype == "bf16" else 10
+    if rows <= 8:
+        return first + size
+    if rows <= 16 or size == 2:
+        return first + 3 + size
+    return first + (6 if -(-rows // 32) <= -(-rows // 48) else 8) + size
+
+
+# (query heads, KV heads, new tokens): 4, 7, 12, 16, 24, 35, 48, 49 and 100 query rows of a KV head
+LAYOUTS = [(8, 2, 1), (14, 2, 1), (6, 2, 4), (8, 2, 4), (12, 2, 4), (14, 2, 5), (24, 2, 4), (14, 2, 7), (40, 2, 5)]
+DIMS = [64, 80, 128, 136, 256, 58, 66, 130, 250]      # the last four put rows off 16-byte boundaries
+CALLS = [(dtype, *layout, dim) for dtype in ("bf16", "f16", "f32") for layout in LAYOUTS for dim in DIMS
+         if dim in (64, 128, 256) or layout in ((8, 2, 1), (14, 2, 5))]
+
+
+def rows_and_width(dtype, heads, kv, new, dim):
+    return new * heads // kv, dim * (4 if dtype == "f32" else 2) % 16 == 0
+
+
+@pytest.mark.parametrize("dtype,heads,kv,new,dim", CALLS)
+def test_attention_every_kernel(ctx, dtype, heads, kv, new, dim):
+    """Three sequences, split over many ranges and joined; then the same ones forty times over, most of them in one
+    range each."""
+    lens = [200, new - 1, 77]
+    cache, g = base.make_cache(ctx, heads + dim, lens, kv, dim, 24, DT[dtype])
+    q = base.queries(g, 3, new, heads, dim, DT[dtype])
+    base.check_attention(ctx, cache, q, lens)
+    many = D.PagedCache(ctx, cache.k_layers, cache.v_layers, cache.block_tables.repeat(40, 1))
+    n = torch.tensor(lens * 40, dtype=torch.int32, device="cuda")
+    out, lse = D.paged_attention(many, 0, q.repeat(40, 1, 1, 1), n, return_lse=True)
+    ctx.sync(60000)
+    ro, rl, to, tl = (x.repeat(40, *[1] * (x.dim() - 1)) for x in base.reference(cache, 0, q, lens))
+    assert bool(((out.double() - ro).abs() <= to + torch.finfo(q.dtype).smallest_normal).all())
+    empty = torch.isneginf(rl)
+    assert torch.equal(torch.isneginf(lse), empty) and bool(((lse.double() - rl).abs()[~empty] <= tl[~empty]).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("heads,dim", [(6, 64), (6, 128), (6, 256), (18, 64), (18, 128), (24, 128), (50, 128), (2, 130), (2, 256)])
+def test_attention_kernels_ignore_what_is_masked(ctx, dtype, heads, dim):
+    base.test_attention_ignores_what_is_masked(ctx, dtype, heads, dim)
+
+
 # -------------------------------------------------------- weights of few bits
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
