@@ -1,9 +1,13 @@
 """verify_tokens at the ends of its numbers: rows of the lowest value, logits and temperatures near the types' limits.
 The reference and its tolerance (none: tokens are whole numbers) are those of ``test_gpu_verify``."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
+from commitllm_b200 import _lib
+from commitllm_b200 import decode as D
 from tests import test_gpu_verify as base
 
 pytestmark = pytest.mark.gpu
@@ -55,3 +59,10 @@ def test_verify_temperatures_at_the_types_ends(ctx, t, with_probs):
         want, _ = base.plain(l.astype(np.float64), drafts, u, temperature)
         drafts[::2, 0] = want[::2, 0]
     base.check(ctx, logits, drafts, u, temperature, probs)
+
+
+def test_verify_workspace_is_what_the_library_asks_for(ctx):
+    for S, k, V in ((1, 0, 1), (3, 4, 128256), (64, 7, 152064), (700, 1, 2), (1, 1, 1 << 20)):
+        out = ctypes.c_size_t()
+        assert _lib.lib().vc_verify_tokens_workspace(ctx.handle, S, k, V, ctypes.byref(out)) == _lib.VC_OK
+        assert out.value == S * (k + 1) * D._VERIFY_ROW_BYTES
