@@ -1160,6 +1160,8 @@ vc_status vc_rope_append(vc_ctx* c, const vc_kv_desc* d, int32_t layer, int32_t 
   vc_status r = check_paged(d, layer, "vc_rope_append");
   if (r) return r;
   if (n_tokens < 0 || n_heads < 1) return fail(VC_EINVAL, "vc_rope_append: n_tokens must be >= 0 and n_heads >= 1");
+  if ((int64_t(n_heads) + 2 * int64_t(d->n_kv_heads)) * d->head_dim > (int64_t(1) << 30))
+    return fail(VC_ENOTSUP, "vc_rope_append: more than 2^30 elements a token");
   if (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > d->head_dim)
     return fail(VC_EINVAL, "vc_rope_append: rotary_dim %d is odd or not in [2, head_dim]", rotary_dim);
   if ((d->n_kv_heads > 1 && d->stride_head < d->head_dim) || (d->block_size > 1 && d->stride_row < d->head_dim))

@@ -413,6 +413,7 @@ VC_API vc_status vc_kv_transcript_commit(vc_ctx* ctx, const vc_kvt_desc* desc, i
  * copied unchanged and no row is written.  Two tokens of one call must not
  * share a row: that row would hold a mix of both.  VC_EINVAL where rows of q_out
  * overlap, or the layer's K and V are one buffer; q_out overlaps no other input.
+ * VC_ENOTSUP for more than 2^30 elements (q, k and v) of one token.
  */
 VC_API vc_status vc_rope_append(vc_ctx* ctx, const vc_kv_desc* cache, int32_t layer, int32_t n_tokens,
                                 const int32_t* positions_dev, const int32_t* seq_ids_dev, int32_t n_heads,

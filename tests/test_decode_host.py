@@ -126,3 +126,16 @@ def test_rope_append_refuses_outputs_that_overlap():
     assert packed_call(_lib.VC_CALL_ROPE_APPEND, [ctypes.addressof(d), 0, 1, 0, 0, 1, 256, 4, 4, 256, 4, 4, 256, 4, 4, 256, 4, 4,
                                                   256, 4, 1.0, 0]) == _lib.VC_EINVAL
     assert "overlap" in _lib.last_error()
+
+
+def test_rope_append_refuses_tokens_past_its_counters():
+    """A token's chunks are counted in 32 bits: 2^30 elements are the most, empty calls on the CPU."""
+    k, v = (ctypes.c_void_p * 1)(256), (ctypes.c_void_p * 1)(512)
+    d = _lib.KvDesc()
+    d.n_layers = d.n_kv_heads = 1
+    d.head_dim, d.dtype, d.n_seqs, d.block_size, d.max_blocks_per_seq = 2, _lib.VC_DTYPE_BF16, 1, 16, 4
+    d.stride_page, d.stride_row, d.stride_head, d.cache_elems, d.block_tables = 32, 2, 2, 512, 256
+    d.k_layers, d.v_layers = (ctypes.cast(p, ctypes.POINTER(ctypes.c_void_p)) for p in (k, v))
+    for heads, want in ((2 ** 29 - 2, _lib.VC_OK), (2 ** 29 - 1, _lib.VC_ENOTSUP), (2 ** 31 - 1, _lib.VC_ENOTSUP)):
+        assert packed_call(_lib.VC_CALL_ROPE_APPEND, [ctypes.addressof(d), 0, 0, 256, 0, heads, 256, 2, 2, 256, 0, 2, 256, 2, 2, 256,
+                                                      2, 2, 256, 2, 1.0, 0]) == want
