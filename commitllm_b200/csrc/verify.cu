@@ -45,10 +45,11 @@ static_assert(32 * sizeof(VerifyPart) <= kVerifyRowBytes, "a row's slices fit it
 
 // How far a keep-or-refuse quantity of the f32 sums may be from its exact value,
 // relative to the row's sum: an exponent of at most 126 (smaller weights are
-// nothing) is rounded three times by 2^-24 of itself, exp2 is off by 2^-22, a
-// thread's sum of at most 2^7 rounded terms by 2^-17, and its at most 12 changes
-// of the maximum by 2^-21 each; 126 * 3 * 2^-24 * ln 2 + 2^-22 + 2^-17 + 12 * 2^-21
-// < 3e-5.
+// nothing) is rounded four times by 2^-24 of itself (log2(e), its quotient by T, the
+// difference of the logits, the product), exp2 is off by 2^-22 in it and at each of
+// three joins (warp, block, row), a thread's sum of at most 2^7 rounded terms by
+// 2^-17, and its at most 12 changes of the maximum by 2^-21 each; 126 * 4 * 2^-24 * ln
+// 2 + 4 * 2^-22 + 2^-17 + 12 * 2^-21 < 3.6e-5.
 constexpr double kOpen = 4e-5;
 // That holds for temperatures in [1e-30, 1e30]: log2(e) / T is then a normal number, and
 // a difference of two logits that passes f32 weighs nothing.  At any other temperature

@@ -14,7 +14,7 @@ What a serving engine does between two commits, on the same
 Lengths, positions, block tables and draws are read on the device, and a call
 allocates only its outputs and workspace (through torch's caching allocator),
 so a step can be captured in a CUDA graph on the context's stream and replayed
-while its tensors change in place.  As everywhere in this package, calls are
+while its tensors change in place.  Serving only: outputs carry no gradients.  As everywhere in this package, calls are
 ordered on the context's stream: inputs made on another stream need that
 stream's work ordered before them.
 """
@@ -314,7 +314,9 @@ def paged_attention(cache: PagedCache, layer: int, q: torch.Tensor, seq_lens: to
     cached rows of each sequence with the new tokens' own (0 or less: a padding row of
     the batch; more than the block table holds: raised by the next ``ctx.sync()``).
     New token j sees rows ``p < seq_lens[s] - n_new + 1 + j``; a token that sees none
-    gets zeros, and what a token does not see cannot reach its output.
+    gets zeros, and what a token does not see cannot reach its output.  Sums are f32
+    in an order that depends on n_new and on the batch's lengths: a token's output
+    may differ in its last bits between batches, not between equal calls.
     ``scale`` defaults to ``head_dim ** -0.5``.  Returns ``out`` (shaped as q),
     or ``(out, lse)`` with the float32 natural log of each softmax's sum
     ``[n_seqs, n_new, n_heads]`` (-inf where nothing is seen), from which shards of
@@ -379,8 +381,8 @@ def verify_tokens(ctx: Context, logits: torch.Tensor, drafts: torch.Tensor, unif
     while ``uniforms[i] * q_i(x_i) < p_i(x_i)``, and the next token is drawn with
     the last uniform from ``max(p - q, 0)`` where a draft was refused, else from
     ``p``.  Without, the token at i is the one ``p_i`` gives for ``uniforms[i]``, and
-    drafts are kept while they equal it: the tokens are then those of one-by-one
-    decoding, whatever was drafted.  A draw from weights w is the lowest v whose
+    drafts are kept while they equal it: the tokens are then those drawn one by one
+    from the same logits, whatever was drafted.  A draw from weights w is the lowest v whose
     running sum passes ``u * sum(w)``.
 
     Returns ``(tokens int32 [n_seqs, n_draft + 1], counts int32 [n_seqs])``: each

@@ -432,8 +432,12 @@ VC_API vc_status vc_rope_append(vc_ctx* ctx, const vc_kv_desc* cache, int32_t la
  * most 2^30 rows a sequence, VC_ENOTSUP otherwise); lse_dev[s][j][h] (NULL:
  * not wanted) = log sum_p exp(scale * q . k_p).  A token that sees no row gets
  * zeros and -infinity; rows a token does not see cannot reach its output,
- * whatever they hold.  Scores, sums and outputs are accumulated in f32 and
- * rounded once.  out: DEVICE [n_seqs][n_new][n_heads][head_dim]; lse: f32
+ * whatever they hold.  An infinity or NaN in a row it does see leaves NaN or infinities
+ * there.  Scores, sums and outputs are accumulated in f32 and rounded once; for
+ * 16-bit rows the weights that multiply V are held to 2^-16 of themselves (bf16) or to
+ * 2^-18 of the largest of their 32 keys (f16), as two 16-bit numbers.  The order of the sums
+ * depends on n_new and on the batch's lengths, so the last bits of a token's
+ * output do too; the same call gives the same bits.  out: DEVICE [n_seqs][n_new][n_heads][head_dim]; lse: f32
  * [n_seqs][n_new][n_heads].  workspace_dev: DEVICE, 16-byte aligned, of at least
  * vc_paged_attention_workspace bytes; a call that may run at the same time (a
  * graph replayed on another stream) needs its own.
@@ -454,7 +458,8 @@ VC_API vc_status vc_paged_attention_workspace(vc_ctx* ctx, const vc_kv_desc* cac
  * <= 2^20): row i is the target's at draft i, row n_draft the one after the last
  * draft.  p_i = softmax(row i / temperature[s]); a temperature not above 0 puts
  * all of p_i on the lowest index of the largest logit.  -infinity rules a token
- * out.  A draw with u from weights w is the lowest v with w_0 + .. + w_v > u *
+ * out; a logit more than 744.44 temperatures below the row's largest weighs nothing
+ * (e^-744.44 is f64's smallest number).  A draw with u from weights w is the lowest v with w_0 + .. + w_v > u *
  * sum(w).
  *
  * draft_probs non-NULL (DEVICE f32 [n_seqs][n_draft][vocab], the distributions
@@ -463,7 +468,7 @@ VC_API vc_status vc_paged_attention_workspace(vc_ctx* ctx, const vc_kv_desc* cac
  * q_i, 0), after the last one kept from p_i, both with uniforms[s][n_draft].
  * draft_probs NULL: the token at position i is drawn from p_i with
  * uniforms[s][i], and x_i is kept while it equals that token; what comes out is
- * then what one-by-one decoding with the same numbers gives, drafts or not.
+ * then what drawing one by one from the same logits and numbers gives, drafts or not.
  * A draft outside [0, vocab) ends the sequence's drafts: the token at its
  * position is drawn from p_i.
  *
