@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attn_tc_ker
 // three, with 92 B/clk of shared memory reads at the HBM's rate, of 128.  Bound by
 // instruction latency, not by the bytes: 35 rows over 16 sequences of up to 8192 (159
 // MB) take 63 us (68 with the queries in registers, which spilled), eight times longer
-// ones 320 us where the bytes take 195 (21 rows: 234); tensor pipe 38 %, 0.37 instructions
+// ones 320 us where the bytes take 195 (21 rows: 234); tensor pipe 42 %, 0.41 instructions
 // a cycle and scheduler, most stalls on fixed latencies.  Two blocks of 16 keys side by
 // side gave 8 % over one.  Row tiles of 8, five warps a scheduler with 96 registers,
 // spilled and took 91 us; leaving out the products of column tiles without a query row
